@@ -143,6 +143,60 @@ int silu_mul_quant(const void *gu, void *q, void *scales, int M, int I, void *st
 /* The same for fp16 (dtype 0) or bf16 (dtype 1). New entry. */
 int vt_silu_mul_quant(const void *gu, void *q, void *scales, int M, int I, int dtype, void *stream);
 
+/* ---- between QKV and o_proj: the step's tables, rotary positions, attention of drafted tokens over a paged cache --
+ * A paged cache is a pair k_cache, v_cache [num_blocks, block_size, Hkv, D] of 16-bit values (any strides with the
+ * last dimension contiguous); slot s is row s % block_size of block s / block_size. block_table [B, width] int32 (row
+ * stride table_stride) lists each request's blocks in order. New entries: the reference leaves these to vLLM. */
+
+/* One step's tables from the requests' lengths, all on the device (int32 unless stated): cached [B] tokens already in
+ * the cache, new_lens [B] tokens of this step (negative: the request has ended). In place: block_table rows gain the
+ * blocks the step needs, held [B] counts each row's blocks, free_blocks [free_cap] is a stack of free block ids of
+ * which the first *free_count are valid (taken from its top in request order; the blocks of ended requests are pushed
+ * afterwards). Written: cu [B + 1] first token row of each request, seq_lens [B] = cached + new, positions, slots,
+ * mask int64 [T] (rows past the last token: 0, -1, 0), *status = OR of 1 free list too short (a request whose blocks
+ * no longer fit, and every one after it, gets none; its tokens without a block have slot -1), 2 a request needs more
+ * blocks than the table is wide (it gets none), 4 more tokens than T, 8 a tree of more than 64 tokens (mask 0 past the
+ * 64th), 16 free_blocks too small for the blocks given back. parents int32 [T] or NULL: index within its request of
+ * each token's parent, -1 for one that follows the context (an index not below the token's own counts as -1); with it
+ * positions are cached + depth and mask gets each token's ancestors and itself; without, the tokens form a chain and
+ * mask is not written. 1 <= B <= 4096. */
+int vt_step_tables(void *block_table, long long table_stride, int width, void *held, void *free_blocks, int free_cap,
+                   void *free_count, const void *cached, const void *new_lens, const void *parents, int B, int T,
+                   int block_size, void *cu, void *seq_lens, void *positions, void *slots, void *mask, void *status,
+                   void *stream);
+
+/* Rotary positions: of each head of q [T, Hq, D] and k [T, Hkv, D] the first rot values are rotated in pairs (i, i +
+ * rot / 2), or (2 i, 2 i + 1) with interleaved, by the angle 2 pi positions[t] turns[i] and multiplied by factor; the
+ * others are copied. transpose != 0: the transposed map (the gradient). positions int64 [T], turns float64 [rot / 2].
+ * Hq or Hkv may be 0; q_out may be q and k_out k. strides (host, in elements): token and head stride of q, q_out, k,
+ * k_out. rot even, <= D and <= 1024. */
+int vt_rotary(const void *q, void *q_out, const void *k, void *k_out, const long long *strides,
+              const void *positions, const void *turns, float factor, int interleaved, int transpose, int T, int Hq,
+              int Hkv, int D, int rot, int dtype, void *stream);
+/* The same for q, with the rotated k and v [T, Hkv, D] written to the paged cache at slots int64 [T] (a slot outside
+ * the cache: that token's k and v are not written). Slots written must differ. strides (host, in elements): token and
+ * head stride of q, q_out, k, v, then block, row and head stride of k_cache and of v_cache. */
+int vt_rotary_cache(const void *q, void *q_out, const void *k, const void *v, void *k_cache, void *v_cache,
+                    const long long *strides, const void *positions, const void *slots, const void *turns,
+                    float factor, int interleaved, int T, int Hq, int Hkv, int D, int rot, long long num_blocks,
+                    int block_size, int dtype, void *stream);
+
+/* Attention of each request's new tokens q [T, Hq, D] over its seq_lens[b] cached keys, the last cu[b + 1] - cu[b] of
+ * which are the new tokens themselves: token i sees every key before those and, of the new tokens, those with their
+ * bit set in mask[cu[b] + i] (int64 [T]), or tokens 0 .. i with mask NULL. Softmax in 32 bits; a token that sees no
+ * key gets 0; keys in blocks whose table entry is outside [0, num_blocks) are not seen, whatever the cache holds
+ * where nothing is seen. Hq a multiple of Hkv (query head h reads cached head h / (Hq / Hkv)), D a multiple of 8 up to
+ * 256, block_size a multiple of 8, caches 16-byte aligned with strides that are multiples of 8 elements, 1 <= max_new
+ * <= 64 (tokens of a request past max_new are not computed; rows past cu[B] are left as they were). strides (host, in
+ * elements): token and head stride of q and out, then block, row and head stride of k_cache and of v_cache. workspace:
+ * vt_tree_attention_ws_bytes bytes, 256-byte aligned, need not be zeroed; calls that may overlap must not share it. */
+size_t vt_tree_attention_ws_bytes(int max_new, int Hq, int Hkv, int D);
+int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, void *out, const long long *strides,
+                      const void *block_table, long long table_stride, int table_width, const void *cu,
+                      const void *seq_lens, const void *mask, int B, int T, int max_new, int Hq, int Hkv, int D,
+                      long long num_blocks, int block_size, float scale, int dtype, void *workspace, size_t ws_bytes,
+                      void *stream);
+
 /* ---- IPC helpers (replace vllm_turing/csrc/ce_ar.cu:77-101, same names and semantics) ------------------------ */
 
 /* A zeroed device buffer of `bytes` and its 64-byte CUDA IPC handle (written to host memory `handle64`).

@@ -21,7 +21,7 @@ _include = os.path.join(os.path.dirname(_here), "include")
 LIB_NAME = "libvllm_turing_b200.so"
 LIB_PATH = os.path.join(_here, LIB_NAME)
 SOURCES = ("w8a8_gemv.cu", "w8a8_tc.cu", "gate_up_silu.cu", "w8a16_tc.cu", "norm_quant.cu", "ar8.cu", "tp_comm.cu",
-           "tp_fused.cu", "tp_prefill.cu", "ref_abi.cu")
+           "tp_fused.cu", "tp_prefill.cu", "ref_abi.cu", "step_tables.cu", "rotary.cu", "tree_attn.cu")
 ARCH = ("-gencode", "arch=compute_100a,code=sm_100a")
 _lib = None
 
@@ -131,6 +131,11 @@ SIGNATURES = {
     "ar8_dequant_sum": (_I, [_P, _P, _I, _P]),
     "vt_ar8_dequant_sum": (_I, [_P, _P, _LL, _I, _P]),
     "vt_silu_mul_quant": (_I, [_P, _P, _P, _I, _I, _I, _P]),
+    "vt_step_tables": (_I, [_P, _LL, _I, _P, _P, _I] + [_P] * 4 + [_I] * 3 + [_P] * 7),
+    "vt_rotary": (_I, [_P] * 7 + [_F] + [_I] * 8 + [_P]),
+    "vt_rotary_cache": (_I, [_P] * 10 + [_F] + [_I] * 6 + [_LL, _I, _I, _P]),
+    "vt_tree_attention_ws_bytes": (_SZ, [_I] * 4),
+    "vt_tree_attention": (_I, [_P] * 6 + [_LL, _I] + [_P] * 3 + [_I] * 6 + [_LL, _I, _F, _I, _P, _SZ, _P]),
     "ce_alloc": (_I, [_SZ, ctypes.POINTER(ctypes.c_void_p), _P]),
     "ce_open": (_I, [_P, ctypes.POINTER(ctypes.c_void_p)]),
     "ce_close": (_I, [_P]),

@@ -1,0 +1,179 @@
+"""Rotary positions of query and key heads (csrc/rotary.cu): pairs by halves or interleaved, part of the head, scaled
+for long contexts; alone (either direction), or in one kernel with the write of k and v to the paged cache.
+
+Angles come from 64-bit frequencies and are reduced in 64 bits, so far positions keep 32-bit accuracy without a table
+of cosines.
+"""
+import ctypes
+import math
+from typing import NamedTuple
+
+import torch
+
+from . import _build
+from ._launch import dtype_code, launch, need, same_device, vector
+
+SCALINGS = ("none", "linear", "ntk", "yarn", "llama3")
+MAX_ROT = 1024
+
+
+class RopeFreqs(NamedTuple):
+    turns: torch.Tensor   # float64 [rot_dim / 2] on the device: turns per position of each pair
+    factor: float         # multiplies the rotated values (yarn's attention factor; 1 otherwise)
+    rot_dim: int
+
+
+def rope_frequencies(rot_dim, base=10000.0, scaling="none", factor=1.0, original_length=None, beta_fast=32.0,
+                     beta_slow=1.0, low_freq_factor=1.0, high_freq_factor=4.0, device="cuda"):
+    """Frequencies base^(-2 i / rot_dim) of the rot_dim / 2 pairs, made once per model, scaled for contexts `factor`
+    times original_length:
+    linear: all divided by factor; ntk: base * factor^(rot_dim / (rot_dim - 2)); yarn: pairs that turn fewer than
+    beta_slow times over original_length divided by factor, those above beta_fast kept, a ramp over the pairs between,
+    rotated values times 0.1 ln(factor) + 1; llama3: wavelengths above original_length / low_freq_factor divided by
+    factor, below original_length / high_freq_factor kept, blended by wavelength between."""
+    need(isinstance(rot_dim, int) and rot_dim >= 0 and rot_dim % 2 == 0 and rot_dim <= MAX_ROT,
+         f"rope_frequencies: rot_dim must be even, 0 .. {MAX_ROT}")
+    need(scaling in SCALINGS, f"rope_frequencies: scaling must be one of {SCALINGS}")
+    need(base > 0 and factor > 0, "rope_frequencies: base and factor must be positive")
+    need(scaling not in ("yarn", "llama3") or (original_length is not None and original_length > 0),
+         f"rope_frequencies: {scaling} needs original_length")
+    need(scaling != "ntk" or rot_dim != 2, "rope_frequencies: ntk needs rot_dim > 2")
+    need(scaling != "yarn" or base != 1.0, "rope_frequencies: yarn needs base != 1")
+    need(scaling != "llama3" or high_freq_factor > low_freq_factor > 0,
+         "rope_frequencies: llama3 needs high_freq_factor > low_freq_factor > 0")
+    if scaling == "ntk":
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    freqs = [base ** (-2.0 * i / rot_dim) for i in range(rot_dim // 2)]
+    scale = 1.0
+    if scaling == "linear":
+        freqs = [f / factor for f in freqs]
+    elif scaling == "yarn" and freqs:
+        def pair_of(turns):   # the pair that makes `turns` turns over original_length
+            return rot_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
+        low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), rot_dim - 1)
+        width = max(high - low, 0.001)
+        ramp = [min(max((i - low) / width, 0.0), 1.0) for i in range(len(freqs))]
+        freqs = [f / factor * r + f * (1.0 - r) for f, r in zip(freqs, ramp)]
+        scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    elif scaling == "llama3":
+        out = []
+        for f in freqs:
+            wave = 2 * math.pi / f
+            s = (original_length / wave - low_freq_factor) / (high_freq_factor - low_freq_factor)
+            s = min(max(s, 0.0), 1.0)
+            out.append((1.0 - s) * f / factor + s * f)
+        freqs = out
+    turns = torch.tensor([f / (2 * math.pi) for f in freqs], dtype=torch.float64, device=device)
+    return RopeFreqs(turns, scale, rot_dim)
+
+
+def _heads(what, x, T, D):
+    need(x.dim() == 3 and x.shape[0] == T and x.shape[2] == D and (x.stride(2) == 1 or x.numel() == 0 or D == 1),
+         f"{what}: [T, heads, D] with a contiguous last dimension, T = {T}, D = {D}, got {tuple(x.shape)} "
+         f"strides {x.stride()}")
+
+
+def _freq_checks(what, freqs, D, positions, T):
+    need(isinstance(freqs, RopeFreqs) and vector(freqs.turns, torch.float64, freqs.rot_dim // 2),
+         f"{what}: freqs must come from rope_frequencies")
+    need(freqs.rot_dim <= D, f"{what}: rotates {freqs.rot_dim} of {D} values")
+    need(vector(positions, torch.int64, T), f"{what}: positions must be contiguous int64 [T]")
+
+
+def rotary(q, k, positions, freqs, interleaved=False, transpose=False, q_out=None, k_out=None):
+    """(q_out, k_out): q [T, Hq, D] and k [T, Hkv, D] (or None) with the first freqs.rot_dim values of each head
+    rotated by positions (int64 [T]); the rest copied. Any token and head strides. q_out / k_out are new tensors unless
+    given; they may be q and k themselves. transpose applies the transposed map: the gradient with respect to the input,
+    given the gradient of the output (and, for factor 1, the rotation back)."""
+    need(q is not None and q.dim() == 3, "rotary: q must be [T, heads, D]")
+    T, Hq, D = q.shape
+    _heads("rotary q", q, T, D)
+    if k is not None:
+        _heads("rotary k", k, T, D)
+    _freq_checks("rotary", freqs, D, positions, T)
+    if q_out is None:
+        q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+    if k is not None and k_out is None:
+        k_out = torch.empty(T, k.shape[1], D, dtype=k.dtype, device=k.device)
+    need(q_out.shape == q.shape and (k is None or k_out.shape == k.shape), "rotary: outputs have the inputs' shapes")
+    _heads("rotary q_out", q_out, T, D)
+    if k is not None:
+        _heads("rotary k_out", k_out, T, D)
+    else:
+        k_out = None
+    code = dtype_code("rotary", q, k, q_out, k_out)
+    dev = same_device("rotary", q, k, positions, freqs.turns, q_out, k_out)
+    Hkv = k.shape[1] if k is not None else 0
+    if T == 0 or Hq + Hkv == 0 or D == 0:
+        return q_out, k_out
+    ks, ko = (k.stride(), k_out.stride()) if k is not None else ((0, 0), (0, 0))
+    qs, qo = q.stride(), q_out.stride()
+    strides = (ctypes.c_longlong * 8)(qs[0], qs[1], qo[0], qo[1], ks[0], ks[1], ko[0], ko[1])
+    launch("vt_rotary", _build.load().vt_rotary, dev, q.data_ptr(), q_out.data_ptr(),
+           k.data_ptr() if k is not None else None, k_out.data_ptr() if k is not None else None, strides,
+           positions.data_ptr(), freqs.turns.data_ptr(), freqs.factor, int(interleaved), int(transpose), T, Hq, Hkv, D,
+           freqs.rot_dim, code)
+    return q_out, k_out
+
+
+def rotary_cache(q, k, v, positions, slots, k_cache, v_cache, freqs, interleaved=False, q_out=None):
+    """q_out: q [T, Hq, D] rotated as by rotary(); k [T, Hkv, D] rotated and v [T, Hkv, D] go to rows slots (int64 [T])
+    of the paged cache k_cache, v_cache [num_blocks, block_size, Hkv, D] (any strides, last dimension contiguous). A
+    token whose slot is outside the cache (step_tables gives -1) writes no k and v. Slots inside it must differ."""
+    need(q is not None and q.dim() == 3, "rotary_cache: q must be [T, heads, D]")
+    T, Hq, D = q.shape
+    _heads("rotary_cache q", q, T, D)
+    _heads("rotary_cache k", k, T, D)
+    _heads("rotary_cache v", v, T, D)
+    Hkv = k.shape[1]
+    need(Hkv >= 1 and v.shape == k.shape, "rotary_cache: k and v must be [T, Hkv, D] alike, Hkv >= 1")
+    need(k_cache.dim() == 4 and v_cache.shape == k_cache.shape and k_cache.shape[1] >= 1
+         and tuple(k_cache.shape[2:]) == (Hkv, D) and (k_cache.numel() == 0 or (k_cache.stride(3) == 1
+                                                                               and v_cache.stride(3) == 1)),
+         f"rotary_cache: the caches must be [num_blocks, block_size, {Hkv}, {D}] with a contiguous last dimension")
+    _freq_checks("rotary_cache", freqs, D, positions, T)
+    need(vector(slots, torch.int64, T), "rotary_cache: slots must be contiguous int64 [T]")
+    if q_out is None:
+        q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+    need(q_out.shape == q.shape, "rotary_cache: q_out has q's shape")
+    _heads("rotary_cache q_out", q_out, T, D)
+    code = dtype_code("rotary_cache", q, k, v, k_cache, v_cache, q_out)
+    dev = same_device("rotary_cache", q, k, v, positions, slots, k_cache, v_cache, freqs.turns, q_out)
+    if T == 0 or D == 0:
+        return q_out
+    qs, qo, ks, vs, kc, vc = q.stride(), q_out.stride(), k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
+    strides = (ctypes.c_longlong * 14)(qs[0], qs[1], qo[0], qo[1], ks[0], ks[1], vs[0], vs[1], kc[0], kc[1], kc[2],
+                                       vc[0], vc[1], vc[2])
+    launch("vt_rotary_cache", _build.load().vt_rotary_cache, dev, q.data_ptr(), q_out.data_ptr(), k.data_ptr(),
+           v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), strides, positions.data_ptr(), slots.data_ptr(),
+           freqs.turns.data_ptr(), freqs.factor, int(interleaved), T, Hq, Hkv, D, freqs.rot_dim, k_cache.shape[0],
+           k_cache.shape[1], code)
+    return q_out
+
+
+_frag = torch.library.Library("vllm_turing", "FRAGMENT")
+_frag.define("rotary_(Tensor(a!) q_out, Tensor(b!)? k_out, Tensor q, Tensor? k, Tensor positions, Tensor turns, "
+             "float factor, bool interleaved, bool transpose) -> ()")
+_frag.define("rotary_cache_(Tensor(a!) q_out, Tensor q, Tensor k, Tensor v, Tensor positions, Tensor slots, "
+             "Tensor(b!) k_cache, Tensor(c!) v_cache, Tensor turns, float factor, bool interleaved) -> ()")
+
+
+@torch.library.impl(_frag, "rotary_", "CUDA")
+def _rotary_op(q_out, k_out, q, k, positions, turns, factor, interleaved, transpose):
+    rotary(q, k, positions, RopeFreqs(turns, factor, 2 * turns.shape[0]), interleaved, transpose, q_out, k_out)
+
+
+@torch.library.impl(_frag, "rotary_cache_", "CUDA")
+def _rotary_cache_op(q_out, q, k, v, positions, slots, k_cache, v_cache, turns, factor, interleaved):
+    rotary_cache(q, k, v, positions, slots, k_cache, v_cache, RopeFreqs(turns, factor, 2 * turns.shape[0]),
+                 interleaved, q_out)
+
+
+@torch.library.register_fake("vllm_turing::rotary_")
+def _rotary_fake(q_out, k_out, q, k, positions, turns, factor, interleaved, transpose):
+    return None
+
+
+@torch.library.register_fake("vllm_turing::rotary_cache_")
+def _rotary_cache_fake(q_out, q, k, v, positions, slots, k_cache, v_cache, turns, factor, interleaved):
+    return None
