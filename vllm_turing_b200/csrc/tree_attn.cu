@@ -4,91 +4,799 @@
 // token i of the request sees every key before those (j < ctx = L - n), and of its own step the tokens whose bit is
 // set in its mask word (bit jj = token jj), or tokens 0 .. i without masks. Out = softmax(scale q K^T) V over the keys
 // it sees, 0 where it sees none. A key in a block whose table entry is out of range is not seen.
+//
+// Rows: the n tokens x G = Hq / Hkv query heads of one cached head share its keys, so they are the rows of one product,
+// 128 to a tile (tcgen05 M = 128; unused rows cost nothing that counts, since rows are independent and the stream of
+// keys bounds the kernel below about 250 rows). Per tile of TK keys:
+//   S [128, TK] = Q K^T       tcgen05 kind::f16, Q and K from shared memory (both K-major, 128-byte swizzle)
+//   P = 2^(S scale log2 e - m) in 16 bits, written to tensor memory; m, l: the row's running maximum and sum (32 bits)
+//   O [128, D] += P V         tcgen05 kind::f16, P from tensor memory, V from shared memory as it lies in the cache
+//                             (keys x D: the "MN-major" operand)
+// O stays in tensor memory for all tiles; a row's m is raised, and O and l rescaled, only when a tile's maximum passes
+// m by more than 8 (a factor 2^8): the quotient O / l is the same, P stays below 2^8 (fp16 P is held 2^7 times larger,
+// so that small weights keep their bits), and rescaling, which reads and writes all of O, is rare.
+//
+// Work: the key tiles of all (request, cached head, row tile) items form one line of units; each CTA (one per SM) takes
+// an equal contiguous range (computed from the lengths on the device, so a captured graph follows them), whatever
+// the lengths. A range that covers part of an item leaves (O, m, l) in the workspace, and a second kernel joins
+// the parts in CTA order. Everything is in a fixed order: same inputs, same bits.
+//
+// CTA: warp 0 loads K and V tiles by TMA through the block table (a box = 64 values x a power of two of rows that
+// divides block_size, so no box crosses a page), a lane per box; warp 1 issues the MMAs; warps 2 .. 5 hold a row a
+// thread. The score MMA of tile t + 1 runs while the softmax of tile t does. Every wait is bounded.
+//
+// What nothing sees must not matter, whatever the memory holds: scores are selected, not added to; in the tiles that
+// reach past ctx the rows of V past L are set to zero in shared memory, and infinities and NaN in the step's own rows
+// are taken out there (0 x inf is NaN) and added to the rows that see them at the end.
 #include <math.h>
 
-#include "common.cuh"
-#include "host_util.h"
+#include "tc_core.cuh"
 
 namespace vt {
 
 constexpr int TA_MAX_NEW = 64;
+constexpr int TA_ROWS = 128;
+constexpr int TA_THREADS = 192;
+constexpr int TA_BARS = 1024;        // barriers and small shared state, bytes
+constexpr int TA_BAD = 16;           // entries of the ring of "pages that are not there" words (>= tiles in flight)
+constexpr float TA_RAISE = 8.0f;     // log2 of the factor by which weights may pass the running maximum
+
+template <int NCH> struct TaLayout {             // NCH: 64-value chunks of the head
+    static constexpr int TK = NCH <= 2 ? 128 : 64;   // keys a tile: 16 .. 32 KB of K
+    static constexpr int DP = NCH * 64;
+    static constexpr int Q_BYTES = NCH * TA_ROWS * 128;
+    static constexpr int SLOT = NCH * TK * 128;
+    static constexpr int S_COL = DP, P_COL = DP + 2 * TK;   // tensor memory: O | S0 S1 | P0 P1
+    static_assert(P_COL + TK <= 512, "tensor memory");
+};
 
 struct TaArgs {
-    const void *q, *k, *v;
+    const void *q, *v;
     void *out;
-    long long q_t, q_h, o_t, o_h, k_b, k_r, k_h, v_b, v_r, v_h;
+    long long q_t, q_h, o_t, o_h, v_b, v_r, v_h;   // strides in elements
     const int *table, *cu, *seq_lens;
     const long long *mask;
     long long table_stride;
-    int width, B, T, max_new, Hq, Hkv, D, bs, num_blocks;
-    float scale;
+    int width, B, T, max_new, Hq, Hkv, G, D, bs, num_blocks;
+    int box_rows;            // rows a TMA box holds
+    int slots;               // ring slots
+    int part_rows;           // rows a part in the workspace has room for
+    int q_vec, o_vec;        // 16-byte accesses fit q / out
+    uint32_t q_flip;         // sign bits to flip (a negative scale)
+    float sl2;               // |scale| log2 e
+    struct TaDesc *desc;     // [grid]
+    float2 *stats;           // [2 grid][part_rows] {m, l}
+    float *parts;            // [2 grid][part_rows][DP]
+    unsigned *status;
+    uint64_t timeout_ns;
 };
 
-// One block per (query token, head): its warps take the keys in turn, each with a running maximum, sum and output.
-template <typename T>
-__global__ void __launch_bounds__(256) tree_attn_simple_kernel(TaArgs A) {
-    __shared__ float sm_o[8][256], sm_m[8], sm_l[8];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int t = blockIdx.x, h = blockIdx.y, hk = h / (A.Hq / A.Hkv);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (t >= A.cu[A.B]) return;
-    int lo = 0, hi = A.B - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (A.cu[mid + 1] > t) hi = mid;
-        else lo = mid + 1;
+// What the joining kernel needs to know of the item that CTA c's range starts inside of.
+struct TaDesc {
+    long long t0, total;     // the item's first unit; units in all
+    int split;               // 1: c's range starts inside an item and c is the first to do so
+    int nt, ge, cu0, n, h, rt, pad;
+};
+
+// ---- the units and a CTA's range of them ---------------------------------------------------------------------------
+struct TaReq {
+    int L, n, cu0, nt, rtn;
+    long long units;
+};
+__device__ __forceinline__ TaReq ta_request(const TaArgs &A, int b, int tk) {
+    TaReq r;
+    r.cu0 = A.cu[b];
+    r.n = max(A.cu[b + 1] - r.cu0, 0);
+    r.L = max(A.seq_lens[b], 0);
+    r.nt = max(1, (int)(((long long)r.L + tk - 1) / tk));
+    r.rtn = (min(r.n, A.max_new) * A.G + TA_ROWS - 1) / TA_ROWS;
+    r.units = (long long)A.Hkv * r.rtn * r.nt;
+    return r;
+}
+
+struct TaPlan {   // in shared memory
+    long long lo, hi, total, base0;
+    int b0, ge;
+};
+
+__device__ __forceinline__ long long ta_range_lo(long long total, int ge, int c) { return total * c / ge; }
+
+struct TaSeg {
+    int b, h, rt, kt0, kt1;
+    TaReq r;
+    long long t0;    // the item's first unit
+    bool head;       // first segment of the CTA
+};
+
+struct TaIter {
+    long long u, hi, base, lo;
+    int b;
+    TaReq r;
+    __device__ __forceinline__ TaIter(const TaArgs &A, const TaPlan &p, int tk)
+        : u(p.lo), hi(p.hi), base(p.base0), lo(p.lo), b(p.b0) {
+        if (u < hi) r = ta_request(A, b, tk);
     }
-    const int b = lo, i = t - A.cu[b], n = A.cu[b + 1] - A.cu[b], L = A.seq_lens[b], ctx = L - n;
-    if (i >= A.max_new) return;
-    const unsigned long long see = A.mask ? (unsigned long long)A.mask[t] : (2ull << i) - 1;
-    const T *q = (const T *)A.q + t * A.q_t + h * A.q_h;
-    float qr[8], o[8], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        qr[e] = lane + 32 * e < A.D ? t2f<T>(q[lane + 32 * e]) * A.scale : 0.0f;
-        o[e] = 0.0f;
+    __device__ __forceinline__ bool next(const TaArgs &A, int tk, TaSeg &s) {
+        if (u >= hi) return false;
+        while (u >= base + r.units) {
+            base += r.units;
+            r = ta_request(A, ++b, tk);
+        }
+        const long long x = u - base, item = x / r.nt;
+        s.b = b;
+        s.r = r;
+        s.kt0 = (int)(x - item * r.nt);
+        s.kt1 = (int)min((long long)r.nt, s.kt0 + (hi - u));
+        s.h = (int)(item / r.rtn);
+        s.rt = (int)(item - (long long)s.h * r.rtn);
+        s.t0 = u - s.kt0;
+        s.head = u == lo;
+        u += s.kt1 - s.kt0;
+        return true;
     }
-    for (int j = warp; j < L; j += 8) {
-        const int jj = j - ctx;
-        if (jj >= 0 && (jj >= 64 || !((see >> jj) & 1))) continue;
-        const int page = j / A.bs;
-        if (page >= A.width) continue;
-        const int blk = A.table[b * A.table_stride + page];
-        if (blk < 0 || blk >= A.num_blocks) continue;
-        const T *k = (const T *)A.k + blk * A.k_b + (j - page * A.bs) * A.k_r + hk * A.k_h;
-        const T *v = (const T *)A.v + blk * A.v_b + (j - page * A.bs) * A.v_r + hk * A.v_h;
-        float s = 0.0f;
+};
+
+// Every thread calls it: total units by a block reduction, then the request that holds the range's first unit.
+__device__ __forceinline__ void ta_plan(const TaArgs &A, int tk, TaPlan *plan, long long *wsum) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (A.B + TA_THREADS - 1) / TA_THREADS, b0 = tid * per, b1 = min(A.B, b0 + per);
+    long long sum = 0;
+    for (int b = b0; b < b1; ++b) sum += ta_request(A, b, tk).units;
+    long long x = sum;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (lane + 32 * e < A.D) s += qr[e] * t2f<T>(k[lane + 32 * e]);
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        const float mn = fmaxf(m, s), mu = mn == -INFINITY ? 0.0f : mn;
-        const float c = expf(m - mu), p = expf(s - mu);
-        l = l * c + p;
-        m = mn;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (lane + 32 * e < A.D) o[e] = o[e] * c + p * t2f<T>(v[lane + 32 * e]);
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
     }
+    if (lane == 31) wsum[warp] = x;
+    __syncthreads();
+    long long before = 0, total = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sm_o[warp][lane + 32 * e] = o[e];
-    if (lane == 0) {
-        sm_m[warp] = m;
-        sm_l[warp] = l;
+    for (int w = 0; w < TA_THREADS / 32; ++w) {
+        if (w < warp) before += wsum[w];
+        total += wsum[w];
+    }
+    const int ge = (int)max(1ll, min((long long)gridDim.x, total));
+    const int c = blockIdx.x;
+    const long long lo = c < ge ? ta_range_lo(total, ge, c) : total, hi = c < ge ? ta_range_lo(total, ge, c + 1) : total;
+    if (tid == 0) {
+        plan->lo = lo;
+        plan->hi = hi;
+        plan->total = total;
+        plan->ge = ge;
+    }
+    long long start = before + x - sum;
+    if (lo < hi && lo >= start && lo < start + sum) {   // exactly one thread
+        int b = b0;
+        for (;; ++b) {
+            const long long u = ta_request(A, b, tk).units;
+            if (lo < start + u) break;
+            start += u;
+        }
+        plan->b0 = b;
+        plan->base0 = start;
     }
     __syncthreads();
-    float mx = -INFINITY, sum = 0.0f, acc = 0.0f;
-    for (int w = 0; w < 8; ++w) mx = fmaxf(mx, sm_m[w]);
-    if (mx == -INFINITY) mx = 0.0f;
-    for (int w = 0; w < 8; ++w) {
-        const float c = expf(sm_m[w] - mx);
-        sum += c * sm_l[w];
-        acc += c * sm_o[w][threadIdx.x];
+}
+
+// ---- small pieces ----------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float ta_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <typename T> __device__ __forceinline__ uint32_t ta_pack(float a, float b);
+template <> __device__ __forceinline__ uint32_t ta_pack<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t ta_pack<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <typename T> __device__ __forceinline__ bool ta_wild(uint32_t half) {
+    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+    return (half & E) == E;
+}
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// V as it lies in the cache, [keys][64 values] rows of 128 bytes: the MMA's N (values) is contiguous, 64-value chunks
+// `chunk` bytes apart (leading offset), groups of 8 keys 1024 bytes apart (stride offset).
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t chunk) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)((chunk >> 4) & 0x3FFFu) << 16;
+    d |= (uint64_t)((1024u >> 4) & 0x3FFFu) << 32;
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)2u << 61;
+    return d;
+}
+// D (TMEM, fp32) (+)= A (smem desc) . B (smem desc)^T, kind::f16
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w,
+                                            uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Bits kk = 0 .. 31: key c0-relative index kk0 + kk is seen, where keys below c0 all are and key c0 + jj has bit jj of
+// `see`.
+__device__ __forceinline__ uint32_t ta_seen(unsigned long long see, int kk0, int c0) {
+    const int jj = kk0 - c0;
+    if (jj <= -32) return 0xffffffffu;
+    if (jj < 0) return (uint32_t)(see << -jj) | ((1u << -jj) - 1u);
+    return jj < 64 ? (uint32_t)(see >> jj) : 0u;
+}
+
+// ---- the kernel ------------------------------------------------------------------------------------------------------
+template <typename T, int NCH>
+__global__ void __launch_bounds__(TA_THREADS, 1)
+    tree_attn_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                     const __grid_constant__ TaArgs A) {
+    using Lay = TaLayout<NCH>;
+    constexpr int TK = Lay::TK;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char *qs = tc_align1024(smem_raw);
+    unsigned char *ring = qs + Lay::Q_BYTES;
+    const int S = A.slots;
+    uint64_t *full = reinterpret_cast<uint64_t *>(ring + (size_t)S * Lay::SLOT);
+    uint64_t *empty = full + S;
+    uint64_t *sfull = empty + S;        // [2] scores in S buffer
+    uint64_t *pfull = sfull + 2;        // [2] weights in P buffer (and V ready for use), the 4 row warps arrive
+    uint64_t *pvdone = pfull + 2;       // [2] the MMAs that read P buffer (and added to O) have completed
+    uint64_t *qfull = pvdone + 2;       // [1] Q in shared memory, the 4 row warps arrive
+    uint64_t *drain = qfull + 1;
+    long long *wsum = reinterpret_cast<long long *>(drain + 1);   // [6]
+    TaPlan *plan = reinterpret_cast<TaPlan *>(wsum + 6);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(plan + 1);
+    volatile int *flags = reinterpret_cast<volatile int *>(tmem_slot + 1);   // [0] abort
+    uint32_t *wild = tmem_slot + 2;                                          // [2 segments][2 words]
+    volatile uint32_t *bad = tmem_slot + 6;                                  // [TA_BAD] 8-row groups not there
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&sfull[b], 1);
+            mbar_init(&pfull[b], 4);
+            mbar_init(&pvdone[b], 1);
+        }
+        mbar_init(qfull, 4);
+        mbar_init(drain, 1);
+        flags[0] = 0;
+        for (int i = 0; i < 4; ++i) wild[i] = 0;
+        fence_mbar_init();
+        tma_prefetch_desc(&tmap_k);
+        tma_prefetch_desc(&tmap_v);
     }
-    if (threadIdx.x < A.D)
-        ((T *)A.out)[t * A.o_t + h * A.o_h + threadIdx.x] = f2t<T>(sum == 0.0f ? 0.0f : acc / sum);
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    pdl_wait();
+    tc_fence_before();
+    ta_plan(A, TK, plan, wsum);   // synchronises the block
+    tc_fence_after();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t *>(tmem_slot);
+    const uint64_t deadline = globaltimer() + A.timeout_ns;
+    TaIter it(A, *plan, TK);
+    TaSeg sg;
+
+    if (warp == 0) {
+        // ---------------- K and V tiles ----------------
+        bool dead = false;
+        int k = 0, g = 0;   // ring position, tile counter
+        const int box = A.box_rows, box_bytes = box * 128;
+        auto load = [&](const CUtensorMap *map, int kt, bool is_k) {
+            const int k0 = kt * TK, s = k % S, live = min(max(sg.r.L - k0, 0), TK);
+            const int boxes = (live + box - 1) / box * NCH;
+            unsigned char *dst = ring + (size_t)s * Lay::SLOT;
+            // the first 32 boxes' pages before the wait: their latency hides behind it
+            auto page_of = [&](int i, int &r0) {
+                const int row = k0 + i / NCH * box, page = row / A.bs;
+                r0 = row - page * A.bs;
+                int blk = page < A.width ? A.table[(long long)sg.b * A.table_stride + page] : -1;
+                return (blk < 0 || blk >= A.num_blocks) ? A.num_blocks : blk;
+            };
+            int r0 = 0, blk = lane < boxes ? page_of(lane, r0) : 0;
+            bool ok = true;
+            if (lane == 0) ok = !flags[0] && mbar_wait(&empty[s], ((uint32_t)(k / S) & 1u) ^ 1u, deadline);
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+            if (!ok) {
+                if (lane == 0) {
+                    if (!flags[0]) report(A.status, ST_PIPE_TIMEOUT | 0x210u);
+                    flags[0] = 1;
+                }
+                dead = true;
+                return;
+            }
+            if (is_k) {
+                uint32_t gone = 0;   // groups of 8 rows whose page is not there (their boxes read as zeros)
+                for (int i = lane; i < boxes; i += 32) {
+                    int r, p = i == lane ? blk : page_of(i, r);
+                    if (p == A.num_blocks) gone |= ((1u << (box / 8)) - 1u) << (i / NCH * (box / 8));
+                }
+                gone = __reduce_or_sync(0xffffffffu, gone);
+                if (lane == 0) bad[g % TA_BAD] = gone;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(boxes * box_bytes));
+            __syncwarp();
+            for (int i = lane; i < boxes; i += 32) {
+                if (i != lane) blk = page_of(i, r0);
+                const int c = i % NCH;
+                tma_load_4d(dst + c * (TK * 128) + i / NCH * box_bytes, map, c * 64, r0, sg.h, blk, &full[s]);
+            }
+            ++k;
+        };
+        while (!dead && it.next(A, TK, sg)) {
+            for (int kt = sg.kt0; kt <= sg.kt1 && !dead; ++kt) {   // K0, K1 V0, K2 V1, .., V last: the order of use
+                if (kt < sg.kt1) load(&tmap_k, kt, true), ++g;
+                if (kt > sg.kt0 && !dead) load(&tmap_v, kt - 1, false);
+            }
+        }
+        if (dead && lane == 0) {   // let the copies already issued land before the shared memory is released
+            const uint64_t d2 = globaltimer() + A.timeout_ns;
+            for (int j = (k > S ? k - S : 0); j < k; ++j) mbar_wait(&full[j % S], (uint32_t)(j / S) & 1u, d2);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        if (lane == 0) {
+            constexpr uint32_t id_s = idesc_f16<T>(TA_ROWS, TK);
+            constexpr uint32_t id_o = idesc_f16<T>(TA_ROWS, Lay::DP) | (1u << 16);   // B (V) is MN-major
+            const int ksteps = (A.D + 15) / 16;
+            int k = 0, g = 0, seg = 0;
+            auto wait = [&](uint64_t *bar, uint32_t parity, unsigned code) {
+                if (!flags[0] && mbar_wait(bar, parity, deadline)) {
+                    tc_fence_after();
+                    return true;
+                }
+                if (!flags[0]) report(A.status, ST_PIPE_TIMEOUT | code);
+                flags[0] = 1;
+                return false;
+            };
+            auto scores = [&](int gt) {   // S[gt] = Q K^T of the ring's next slot
+                const int s = k % S;
+                if (!wait(&full[s], (uint32_t)(k / S) & 1u, 0x220u)) return false;
+                const uint32_t kb = smem_u32(ring + (size_t)s * Lay::SLOT), qb = smem_u32(qs);
+                const uint32_t d = tmem_base + Lay::S_COL + (uint32_t)((gt & 1) * TK);
+                for (int i = 0; i < ksteps; ++i)
+                    umma_f16(d, sw128_desc(qb + (i >> 2) * (TA_ROWS * 128)) + 2 * (i & 3),
+                             sw128_desc(kb + (i >> 2) * (TK * 128)) + 2 * (i & 3), id_s, i > 0);
+                umma_commit(&sfull[gt & 1]);
+                umma_commit(&empty[s]);
+                ++k;
+                return true;
+            };
+            bool ok = true;
+            while (ok && it.next(A, TK, sg)) {
+                const int N = sg.kt1 - sg.kt0;
+                ok = wait(qfull, (uint32_t)seg & 1u, 0x230u) && scores(g);
+                for (int t = 0; ok && t < N; ++t, ++g) {
+                    if (t + 1 < N) ok = scores(g + 1);
+                    ok = ok && wait(&pfull[g & 1], (uint32_t)(g >> 1) & 1u, 0x240u);
+                    const int s = k % S;
+                    ok = ok && wait(&full[s], (uint32_t)(k / S) & 1u, 0x250u);
+                    if (!ok) break;
+                    const uint32_t p = tmem_base + Lay::P_COL + (uint32_t)((g & 1) * (TK / 2));
+                    const uint64_t v = sw128_mn_desc(smem_u32(ring + (size_t)s * Lay::SLOT), TK * 128);
+#pragma unroll
+                    for (int i = 0; i < TK / 16; ++i)   // 16 keys a step: 8 columns of P, 2048 bytes of V
+                        umma_f16_ts(tmem_base, p + 8 * i, v + 128 * i, id_o, (t > 0 || i > 0) ? 1u : 0u);
+                    umma_commit(&pvdone[g & 1]);
+                    umma_commit(&empty[s]);
+                    ++k;
+                }
+                ++seg;
+            }
+            umma_commit(drain);   // every MMA issued has completed once it flips
+            mbar_wait(drain, 0u, globaltimer() + A.timeout_ns);
+        }
+        __syncwarp();
+    } else {
+        // ---------------- rows: softmax and output ----------------
+        const int q4 = warp & 3, row = q4 * 32 + lane, tid = q4 * 32 + lane;
+        const uint32_t lane_base = tmem_base + ((uint32_t)(q4 * 32) << 16);
+        bool dead = false;
+        auto wait = [&](uint64_t *bar, uint32_t parity, unsigned code) {
+            if (dead) return;   // the loops go on without data, so that the barriers among these warps stay matched
+            if (__any_sync(0xffffffffu, flags[0] != 0) || !warp_wait(bar, parity, deadline)) {
+                if (lane == 0 && !flags[0]) report(A.status, ST_PIPE_TIMEOUT | code);
+                flags[0] = 1;
+                dead = true;
+            }
+            tc_fence_after();
+        };
+        auto load_q = [&](const TaSeg &s) {   // the item's rows, swizzled as TMA would lay them out
+            constexpr int NV = NCH * 8;
+            const int live = min(min(s.r.n, A.max_new) * A.G - s.rt * TA_ROWS, TA_ROWS);
+            for (int idx = tid; idx < live * NV; idx += 128) {
+                const int r = idx / NV, v = idx - r * NV, gr = s.rt * TA_ROWS + r, i = gr / A.G;
+                const int tok = s.r.cu0 + i, d = v * 8;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (d < A.D && tok >= 0 && tok < A.T) {
+                    const T *src = reinterpret_cast<const T *>(A.q) + (long long)tok * A.q_t +
+                                   (long long)(s.h * A.G + gr - i * A.G) * A.q_h + d;
+                    if (A.q_vec) {
+                        x = *reinterpret_cast<const uint4 *>(src);
+                    } else {
+                        const uint16_t *e = reinterpret_cast<const uint16_t *>(src);
+                        x = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
+                                       e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+                    }
+                    x = make_uint4(x.x ^ A.q_flip, x.y ^ A.q_flip, x.z ^ A.q_flip, x.w ^ A.q_flip);
+                }
+                *reinterpret_cast<uint4 *>(qs + (v >> 3) * (TA_ROWS * 128) + r * 128 + (((v & 7) ^ (r & 7)) << 4)) = x;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(qfull);
+        };
+        int g = 0, kbase = 0, seg = 0;
+        bool has = it.next(A, TK, sg);
+        if (threadIdx.x == 64) A.desc[blockIdx.x].split = 0;
+        if (has) {
+            if (threadIdx.x == 64 && sg.kt0 > 0) {
+                TaDesc d;
+                d.t0 = sg.t0;
+                d.total = plan->total;
+                d.split = sg.t0 >= ta_range_lo(plan->total, plan->ge, blockIdx.x - 1);
+                d.nt = sg.r.nt;
+                d.ge = plan->ge;
+                d.cu0 = sg.r.cu0;
+                d.n = sg.r.n;
+                d.h = sg.h;
+                d.rt = sg.rt;
+                d.pad = 0;
+                A.desc[blockIdx.x] = d;
+            }
+            load_q(sg);
+        }
+        while (has) {
+            const int ctx = sg.r.L - sg.r.n, N = sg.kt1 - sg.kt0;
+            const int live = min(min(sg.r.n, A.max_new) * A.G - sg.rt * TA_ROWS, TA_ROWS);
+            const int gr = sg.rt * TA_ROWS + row, tok_i = gr / A.G, tok = sg.r.cu0 + tok_i;
+            const bool mine = row < live && tok >= 0 && tok < A.T;
+            const bool warp_live = q4 * 32 < live;
+            unsigned long long see = 0;
+            if (mine) {
+                see = A.mask ? (unsigned long long)A.mask[tok] : (2ull << tok_i) - 1ull;
+                if (sg.r.n < 64) see &= (1ull << sg.r.n) - 1ull;
+            }
+            float m = -INFINITY, l = 0.0f;
+            for (int t = 0; t < N; ++t, ++g) {
+                const int k0 = (sg.kt0 + t) * TK, buf = g & 1;
+                const uint32_t use = (uint32_t)(g >> 1);
+                const bool past = k0 + TK > ctx;
+                wait(&sfull[buf], use & 1u, 0x260u);
+                const uint32_t gone = bad[g % TA_BAD];
+                float x[TK];
+                if (warp_live) {
+#pragma unroll
+                    for (int c = 0; c < TK; c += 32)
+                        tmem_ld32(lane_base + Lay::S_COL + (uint32_t)(buf * TK + c),
+                                  *reinterpret_cast<uint32_t(*)[32]>(&x[c]));
+                    tmem_ld_wait();
+                    const bool masked = past || gone != 0;
+                    if (masked) {
+#pragma unroll
+                        for (int c = 0; c < TK; c += 32) {
+                            uint32_t vis = ta_seen(see, k0 + c, ctx);
+                            const uint32_t g4 = (gone >> (c / 8)) & 15u;
+                            vis &= ~(((g4 * 0x00204081u) & 0x01010101u) * 255u);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) x[c + j] = (vis >> j) & 1u ? x[c + j] : -INFINITY;
+                        }
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int j = 0; j < TK; ++j) mx[j & 3] = fmaxf(mx[j & 3], x[j]);
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    const float tm = top == -INFINITY ? -INFINITY : top * A.sl2;
+                    const bool raise = tm > m + TA_RAISE || (m == -INFINITY && tm > m);
+                    if (__any_sync(0xffffffffu, raise)) {
+                        const float f = raise ? ta_exp2(m - tm) : 1.0f;
+                        if (raise) m = tm;
+                        l *= f;
+                        if (t > 0) {   // O of the tiles before this one
+                            wait(&pvdone[(g - 1) & 1], (uint32_t)((g - 1) >> 1) & 1u, 0x270u);
+#pragma unroll 1
+                            for (int c = 0; c < Lay::DP; c += 32) {
+                                uint32_t o[32];
+                                tmem_ld32(lane_base + (uint32_t)c, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                                tmem_st32(lane_base + (uint32_t)c, o);
+                            }
+                            tmem_st_wait();
+                        }
+                    }
+                    constexpr float BIAS = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+                    const float off = (m == -INFINITY ? 0.0f : -m) + BIAS;
+                    if (t > 1 || g > 1)   // the MMAs that read this P buffer two tiles ago
+                        wait(&pvdone[buf], (use & 1u) ^ 1u, 0x280u);
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int c = 0; c < TK; c += 64) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int j = 0; j < 64; j += 2) {
+                            // a hidden key's score is -inf: 2^-inf = 0 (with scale 0, -inf x 0 would be NaN: selected)
+                            const float a = x[c + j] == -INFINITY ? 0.0f : ta_exp2(__fmaf_rn(x[c + j], A.sl2, off));
+                            const float b =
+                                x[c + j + 1] == -INFINITY ? 0.0f : ta_exp2(__fmaf_rn(x[c + j + 1], A.sl2, off));
+                            sum[j & 2] += a;
+                            sum[(j & 2) + 1] += b;
+                            w[j >> 1] = ta_pack<T>(a, b);
+                        }
+                        tmem_st32(lane_base + Lay::P_COL + (uint32_t)(buf * (TK / 2) + c / 2), w);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_st_wait();
+                }
+                if (past) {
+                    // rows of V that not every row sees: zeros past the length, no infinities or NaN before it
+                    const int vi = kbase + (t + 1 < N ? 2 * t + 2 : 2 * N - 1), r0 = max(ctx - k0, 0);
+                    wait(&full[vi % S], (uint32_t)(vi / S) & 1u, 0x290u);
+                    unsigned char *vs = ring + (size_t)(vi % S) * Lay::SLOT;
+                    for (int idx = tid; idx < (TK - r0) * NCH * 8 && !dead; idx += 128) {
+                        const int r = r0 + idx / (NCH * 8), v = idx % (NCH * 8), j = k0 + r;
+                        uint4 *p = reinterpret_cast<uint4 *>(vs + (v >> 3) * (TK * 128) + r * 128 +
+                                                             (((v & 7) ^ (r & 7)) << 4));
+                        if (j >= sg.r.L) {
+                            *p = make_uint4(0, 0, 0, 0);
+                            continue;
+                        }
+                        uint4 y = *p;
+                        uint32_t *w = reinterpret_cast<uint32_t *>(&y);
+                        bool any = false;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (ta_wild<T>(w[e])) w[e] &= 0xffff0000u, any = true;
+                            if (ta_wild<T>(w[e] >> 16)) w[e] &= 0x0000ffffu, any = true;
+                        }
+                        if (any) {
+                            *p = y;
+                            const int jj = j - ctx;   // < n; a wild one past the mask's 64 bits is seen by no row
+                            if (jj < 64) atomicOr(&wild[(seg & 1) * 2 + (jj >> 5)], 1u << (jj & 31));
+                        }
+                    }
+                    fence_proxy_async();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pfull[buf]);
+            }
+            kbase += 2 * N;
+            // the next item's Q may go in: this one's last scores are done
+            const TaSeg cur = sg;
+            has = it.next(A, TK, sg);
+            if (has) load_q(sg);
+            wait(&pvdone[(g - 1) & 1], (uint32_t)((g - 1) >> 1) & 1u, 0x2a0u);
+            if (threadIdx.x == 64) {
+                wild[((seg & 1) ^ 1) * 2] = 0;
+                wild[((seg & 1) ^ 1) * 2 + 1] = 0;
+            }
+            named_sync(TC_EPI_BAR, 128);
+            if (warp_live) {
+                const volatile uint32_t *wv = wild + (seg & 1) * 2;
+                const unsigned long long wn = see & (wv[0] | (unsigned long long)wv[1] << 32);
+                const bool whole = cur.kt0 == 0 && cur.kt1 == cur.r.nt;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const size_t prow = (size_t)(2 * blockIdx.x + (cur.head ? 0 : 1)) * A.part_rows + row;
+                T *dst = reinterpret_cast<T *>(A.out) + (long long)tok * A.o_t +
+                         (long long)(cur.h * A.G + gr - tok_i * A.G) * A.o_h;
+#pragma unroll 1
+                for (int c = 0; c < Lay::DP; c += 32) {
+                    float o[32];
+                    tmem_ld32(lane_base + (uint32_t)c, *reinterpret_cast<uint32_t(*)[32]>(o));
+                    tmem_ld_wait();
+                    if (!mine || dead) continue;
+                    if (wn) {   // the values taken out above, for the rows that see them
+                        for (unsigned long long left = wn; left; left &= left - 1) {
+                            const int j = ctx + __ffsll((long long)left) - 1, page = j / A.bs;
+                            if (j < cur.kt0 * TK || j >= cur.kt1 * TK || page >= A.width) continue;
+                            const int blk = A.table[(long long)cur.b * A.table_stride + page];
+                            if (blk < 0 || blk >= A.num_blocks) continue;
+                            const T *v = reinterpret_cast<const T *>(A.v) + blk * A.v_b + (j - page * A.bs) * A.v_r + cur.h * A.v_h;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                if (c + e >= A.D) break;
+                                const float f = t2f<T>(v[c + e]);
+                                if (!isfinite(f)) o[e] += f;
+                            }
+                        }
+                    }
+                    if (!whole) {
+                        float4 *w = reinterpret_cast<float4 *>(A.parts + prow * Lay::DP + c);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            w[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            if (c + e >= A.D) break;
+                            uint32_t w[4];
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) w[h] = ta_pack<T>(o[e + 2 * h] * inv, o[e + 2 * h + 1] * inv);
+                            if (A.o_vec) {
+                                *reinterpret_cast<uint4 *>(dst + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                            } else {
+                                uint16_t *d16 = reinterpret_cast<uint16_t *>(dst + c + e);
+#pragma unroll
+                                for (int h = 0; h < 4; ++h) {
+                                    d16[2 * h] = (uint16_t)w[h];
+                                    d16[2 * h + 1] = (uint16_t)(w[h] >> 16);
+                                }
+                            }
+                        }
+                    }
+                }
+                if (!whole && mine) A.stats[prow] = make_float2(m, l);
+            }
+            tc_fence_before();
+            ++seg;
+        }
+    }
+    // all roles done: free TMEM after every TMEM access and MMA of the CTA has completed
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// Joins the parts of the items that a range boundary cuts: block (c - 1, chunk of rows) for the item that CTA c's
+// range starts inside of, when c is the first such CTA. Contributors are CTAs c - 1 .. c1 in order; WPR warps share a
+// row's contributors and add up in warp order.
+constexpr int TJ_THREADS = 512;
+template <typename T, int NCH, int WPR>
+__global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_constant__ TaArgs A) {
+    constexpr int DP = NCH * 64, RPB = TJ_THREADS / 32 / WPR, E = DP / 32;
+    __shared__ float acc_sm[RPB][WPR > 1 ? WPR - 1 : 1][DP];
+    __shared__ float l_sm[RPB][WPR];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int c = blockIdx.x + 1;
+    const TaDesc d = A.desc[c];
+    if (!d.split) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rb = warp / WPR, wr = warp % WPR;
+    const int r = blockIdx.y * RPB + rb;
+    const int gr = d.rt * TA_ROWS + r, i = gr / A.G, tok = d.cu0 + i;
+    const bool mine = r < min(min(d.n, A.max_new) * A.G - d.rt * TA_ROWS, TA_ROWS) && tok >= 0 && tok < A.T;
+    const int first = (d.t0 == ta_range_lo(d.total, d.ge, c - 1)) ? 2 * (c - 1) : 2 * (c - 1) + 1;
+    int c1 = (int)((d.t0 + d.nt - 1) * d.ge / d.total);   // the CTA holding the item's last unit
+    while (c1 + 1 < d.ge && ta_range_lo(d.total, d.ge, c1 + 1) <= d.t0 + d.nt - 1) ++c1;
+    const int nc = c1 - (c - 1) + 1;
+    auto slot = [&](int j) { return (size_t)(j == 0 ? first : 2 * (c - 1 + j)) * A.part_rows + r; };
+    float M = -INFINITY;
+    if (mine)
+        for (int j = lane; j < nc; j += 32) M = fmaxf(M, A.stats[slot(j)].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if (M == -INFINITY) M = 0.0f;
+    float acc[E], l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+    if (mine) {
+#pragma unroll 4
+        for (int j = wr; j < nc; j += WPR) {
+            const size_t s = slot(j);
+            const float2 st = A.stats[s];
+            const float w = ta_exp2(st.x - M);
+            l += w * st.y;
+            const float2 *p = reinterpret_cast<const float2 *>(A.parts + s * DP);
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float2 v = p[lane + 16 * e];
+                if (w != 0.0f) {
+                    acc[e] = __fmaf_rn(w, v.x, acc[e]);
+                    acc[e + 1] = __fmaf_rn(w, v.y, acc[e + 1]);
+                }
+            }
+        }
+    }
+    if (WPR > 1) {
+        if (wr > 0) {
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                acc_sm[rb][wr - 1][2 * lane + 32 * e] = acc[e];
+                acc_sm[rb][wr - 1][2 * lane + 32 * e + 1] = acc[e + 1];
+            }
+        }
+        if (lane == 0) l_sm[rb][wr] = l;
+        __syncthreads();
+        if (wr > 0) return;
+#pragma unroll
+        for (int w = 1; w < WPR; ++w) {
+            l += l_sm[rb][w];
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                acc[e] += acc_sm[rb][w - 1][2 * lane + 32 * e];
+                acc[e + 1] += acc_sm[rb][w - 1][2 * lane + 32 * e + 1];
+            }
+        }
+    }
+    if (!mine) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T *dst = reinterpret_cast<T *>(A.out) + (long long)tok * A.o_t + (long long)(d.h * A.G + gr - i * A.G) * A.o_h;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+        const int col = 2 * lane + 32 * e;
+        if (col >= A.D) continue;
+        dst[col] = f2t<T>(acc[e] * inv);
+        dst[col + 1] = f2t<T>(acc[e + 1] * inv);
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+// [num_blocks][heads][rows][D] of 16-bit values with any strides (elements, multiples of 8); a box is 64 values of
+// `box_rows` rows; what lies outside reads as 0.
+static bool ta_map(CUtensorMap *m, const void *base, int D, int bs, int Hkv, int nb, long long sr, long long sh,
+                   long long sb, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)bs, (cuuint64_t)Hkv, (cuuint64_t)nb};
+    cuuint64_t strides[3] = {(cuuint64_t)sr * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
+    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static int ta_part_rows(int max_new, int G) { return max_new * G < TA_ROWS ? max_new * G : TA_ROWS; }
+static size_t ta_desc_bytes(int grid) { return ((size_t)grid * sizeof(TaDesc) + 255) & ~(size_t)255; }
+static size_t ta_stats_bytes(int grid, int rows) { return ((size_t)2 * grid * rows * sizeof(float2) + 255) & ~(size_t)255; }
+
+template <typename T, int NCH> static int launch_ta(const CUtensorMap &mk, const CUtensorMap &mv, TaArgs A, cudaStream_t s) {
+    using Lay = TaLayout<NCH>;
+    const int dev = cur_device();
+    if (dev < 0 || dev >= VT_MAX_DEV) return VT_EARG;
+    int slots = (max_smem_optin(dev) - 1024 - TA_BARS - Lay::Q_BYTES) / Lay::SLOT;
+    if (slots > 12) slots = 12;
+    if (slots < 4) return VT_EARG;
+    A.slots = slots;
+    const int smem = 1024 + Lay::Q_BYTES + slots * Lay::SLOT + TA_BARS;
+    static std::atomic<bool> attr[VT_MAX_DEV];
+    if (!attr[dev]) {
+        if (cudaFuncSetAttribute(tree_attn_kernel<T, NCH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+            cudaSuccess)
+            return (int)cudaGetLastError();
+        attr[dev] = true;
+    }
+    const int grid = num_sms(dev);
+    if (int rc = launch_k(tree_attn_kernel<T, NCH>, dim3(grid), dim3(TA_THREADS), smem, s, true, mk, mv, A)) return rc;
+    if (grid < 2) return 0;
+    if (A.part_rows <= 32)
+        return launch_k(tree_join_kernel<T, NCH, 4>, dim3(grid - 1, (A.part_rows + 3) / 4), dim3(TJ_THREADS), 0, s, true,
+                        A);
+    return launch_k(tree_join_kernel<T, NCH, 1>, dim3(grid - 1, (A.part_rows + 15) / 16), dim3(TJ_THREADS), 0, s, true,
+                    A);
+}
+
+template <typename T> static int dispatch_ta(const CUtensorMap &mk, const CUtensorMap &mv, const TaArgs &A, cudaStream_t s) {
+    if (A.D <= 64) return launch_ta<T, 1>(mk, mv, A, s);
+    if (A.D <= 128) return launch_ta<T, 2>(mk, mv, A, s);
+    if (A.D <= 192) return launch_ta<T, 3>(mk, mv, A, s);
+    return launch_ta<T, 4>(mk, mv, A, s);
 }
 
 }  // namespace vt
@@ -98,11 +806,9 @@ using namespace vt;
 extern "C" {
 
 size_t vt_tree_attention_ws_bytes(int max_new, int Hq, int Hkv, int D) {
-    (void)max_new;
-    (void)Hq;
-    (void)Hkv;
-    (void)D;
-    return 256;
+    if (max_new < 1 || max_new > TA_MAX_NEW || Hkv < 1 || Hq < Hkv || D < 1 || D > 256) return 0;
+    const int grid = num_sms(cur_device()), rows = ta_part_rows(max_new, Hq / Hkv), dp = (D + 63) / 64 * 64;
+    return ta_desc_bytes(grid) + ta_stats_bytes(grid, rows) + (size_t)2 * grid * rows * dp * sizeof(float);
 }
 
 int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, void *out, const long long *strides,
@@ -111,22 +817,33 @@ int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, v
                       long long num_blocks, int block_size, float scale, int dtype, void *workspace, size_t ws_bytes,
                       void *stream) {
     if (!q || !k_cache || !v_cache || !out || !strides || !block_table || !cu || !seq_lens || B < 1 || T < 0 ||
-        max_new < 1 || max_new > TA_MAX_NEW || Hkv < 1 || Hq < Hkv || Hq % Hkv || D < 8 || D > 256 || D % 8 ||
-        block_size < 8 || block_size % 8 || table_width < 0 || num_blocks < 0 || (dtype != 0 && dtype != 1) ||
-        !workspace || ws_bytes < vt_tree_attention_ws_bytes(max_new, Hq, Hkv, D))
+        max_new < 1 || max_new > TA_MAX_NEW || Hkv < 1 || Hq < Hkv || Hq % Hkv || Hq > (1 << 20) || D < 8 || D > 256 ||
+        D % 8 || block_size < 8 || block_size % 8 || table_width < 0 || num_blocks < 1 || num_blocks > 0x7ffffffe ||
+        (dtype != 0 && dtype != 1) || !workspace || ((uintptr_t)workspace & 255) ||
+        ws_bytes < vt_tree_attention_ws_bytes(max_new, Hq, Hkv, D) || ((uintptr_t)k_cache & 15) ||
+        ((uintptr_t)v_cache & 15) || !(scale == scale))
         return VT_EARG;
+    for (int i = 4; i < 10; ++i)
+        if (strides[i] < 0 || strides[i] % 8) return VT_EARG;
+    if (T == 0) return 0;
+    cudaStream_t s = (cudaStream_t)stream;
+    void *scratch;
     TaArgs A{};
+    if (int rc = ws_acquire(0, s, &scratch, &A.status)) return rc;
+    int box = 8;   // the largest power of two of rows that divides the block, at most a tile
+    const int tk = D <= 128 ? 128 : 64;
+    while (box * 2 <= tk && block_size % (box * 2) == 0) box *= 2;
+    CUtensorMap mk, mv;
+    if (!ta_map(&mk, k_cache, D, block_size, Hkv, (int)num_blocks, strides[5], strides[6], strides[4], box) ||
+        !ta_map(&mv, v_cache, D, block_size, Hkv, (int)num_blocks, strides[8], strides[9], strides[7], box))
+        return VT_EARG;
     A.q = q;
-    A.k = k_cache;
     A.v = v_cache;
     A.out = out;
     A.q_t = strides[0];
     A.q_h = strides[1];
     A.o_t = strides[2];
     A.o_h = strides[3];
-    A.k_b = strides[4];
-    A.k_r = strides[5];
-    A.k_h = strides[6];
     A.v_b = strides[7];
     A.v_r = strides[8];
     A.v_h = strides[9];
@@ -141,15 +858,24 @@ int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, v
     A.max_new = max_new;
     A.Hq = Hq;
     A.Hkv = Hkv;
+    A.G = Hq / Hkv;
     A.D = D;
     A.bs = block_size;
     A.num_blocks = (int)num_blocks;
-    A.scale = scale;
-    if (T == 0) return 0;
-    cudaStream_t s = (cudaStream_t)stream;
-    const dim3 grid(T, Hq);
-    if (dtype == 0) return launch_k(tree_attn_simple_kernel<__half>, grid, dim3(256), 0, s, true, A);
-    return launch_k(tree_attn_simple_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, true, A);
+    A.box_rows = box;
+    A.q_vec = ((uintptr_t)q & 15) == 0 && ((A.q_t | A.q_h) & 7) == 0;
+    A.o_vec = ((uintptr_t)out & 15) == 0 && ((A.o_t | A.o_h) & 7) == 0;
+    A.q_flip = scale < 0.0f ? 0x80008000u : 0u;
+    A.sl2 = fabsf(scale) * 1.4426950408889634f;
+    A.part_rows = ta_part_rows(max_new, A.G);
+    A.timeout_ns = pipe_timeout_ns();
+    const int grid = num_sms(cur_device());
+    char *ws = (char *)workspace;
+    A.desc = (TaDesc *)ws;
+    A.stats = (float2 *)(ws + ta_desc_bytes(grid));
+    A.parts = (float *)(ws + ta_desc_bytes(grid) + ta_stats_bytes(grid, A.part_rows));
+    if (dtype == 0) return dispatch_ta<__half>(mk, mv, A, s);
+    return dispatch_ta<__nv_bfloat16>(mk, mv, A, s);
 }
 
 }  // extern "C"

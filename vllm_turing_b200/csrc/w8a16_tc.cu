@@ -85,35 +85,6 @@ struct WhArgs {
     int ldo;    // output row stride in elements (>= N)
 };
 
-// D (TMEM, fp32) (+)= A (TMEM, 16-bit) . B (shared-memory descriptor)^T, kind::f16
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// Instruction descriptor, kind::f16: fp32 accumulator (bits 4-5 = 1), A and B both bf16 (bits 7-9, 10-12 = 1) or
-// both fp16 (0), both K-major, MMA M x N.
-template <typename T> __host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
-    constexpr uint32_t ab = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    return (1u << 4) | (ab << 7) | (ab << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-// 32 consecutive 32-bit TMEM columns of the warp's 32 lanes (thread i writes lane base + i)
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
 // Four int8 (one word, element k in the low byte) -> two words of 16-bit floats {k, k+1}, {k+2, k+3} (element k in the
 // low half), exactly. The bytes are first spread to 0x00b1_00b0 / 0x00b3_00b2.
 //   bf16: with b = v - 128 s (v = b & 127, s = the sign bit), 0x4300 | v is bf16(128 + v) and 0x4300 | (b & 128) is
@@ -135,11 +106,6 @@ template <> __device__ __forceinline__ uint32_t cvt_pair<__half>(uint32_t p) {
 template <typename T> __device__ __forceinline__ void cvt_word(uint32_t w, uint32_t &o0, uint32_t &o1) {
     o0 = cvt_pair<T>(__byte_perm(w, 0u, 0x4140));
     o1 = cvt_pair<T>(__byte_perm(w, 0u, 0x4342));
-}
-
-// all lanes of the warp wait on the same barrier; the warp continues only if every lane saw it complete
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, uint64_t deadline) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, deadline)) != 0;
 }
 
 template <typename T, int BN, int NW>
