@@ -31,9 +31,10 @@
 // the lengths. A range that covers part of an item leaves (O, m, l) in the workspace, and a second kernel joins
 // the parts in CTA order. Everything is in a fixed order: same inputs, same bits.
 //
-// CTA: warp 0 loads K and V tiles by TMA through the block table (a box holds a power of two of rows that divides
-// block_size, so no box crosses a page), a lane per box; warp 1 issues the MMAs; the others hold rows. The score MMA of
-// tile t + 1 runs while the softmax of tile t does. Every wait is bounded.
+// CTA: the first warps hold rows; one warp each loads K and V tiles by TMA through the block table (a box holds a power
+// of two of rows that divides block_size, so no box crosses a page), a lane per box, into two rings; one issues the
+// MMAs. The K warp walks the CTA's range and leaves each segment (an item's tiles in the range) in shared memory for
+// the others. The score MMA of tile t + 1 runs while the softmax of tile t does. Every wait is bounded.
 //
 // What nothing sees must not matter, whatever the memory holds: scores are selected, not added to; in the tiles that
 // reach past ctx the rows of V past L are set to zero in shared memory, and infinities and NaN in the step's own rows
@@ -46,8 +47,9 @@ namespace vt {
 
 constexpr int TA_MAX_NEW = 64;
 constexpr int TA_ROWS = 128;
-constexpr int TA_BARS = 2048;        // barriers and small shared state, bytes
-constexpr int TA_BAD = 16;           // entries of the ring of "pages that are not there" words (>= tiles in flight)
+constexpr int TA_BARS = 3072;        // barriers and small shared state, bytes
+constexpr int TA_RING = 16;          // entries of the rings of segments and of "pages that are not there" words: more
+                                     // than the tiles between the K warp and the rows (at most 6 slots + 4)
 constexpr float TA_RAISE = 8.0f;     // log2 of the factor by which weights may pass the running maximum
 
 template <int NCH, int REP> struct TaLayout {        // NCH: 64-value chunks of the head
@@ -55,7 +57,7 @@ template <int NCH, int REP> struct TaLayout {        // NCH: 64-value chunks of 
     static constexpr int DP = NCH * 64;
     static constexpr int CH = REP == 1 && NCH <= 2 ? 2 : 1;
     static constexpr bool QT = CH == 1;                            // Q in tensor memory
-    static constexpr int THREADS = 64 + 128 * CH;
+    static constexpr int THREADS = 128 * CH + 128;                 // rows, then the K, MMA and V warps and a spare
     static constexpr int Q_BYTES = QT ? 0 : NCH * TA_ROWS * 128;
     static constexpr int STAGE_LD = 33;                            // floats a row of the staging area
     static constexpr int STAGE = REP > 1 ? (TA_ROWS * STAGE_LD * 4 + 1023) / 1024 * 1024 : 0;
@@ -75,7 +77,7 @@ struct TaArgs {
     int box_rows;            // rows a TMA box holds
     int fold, head_step;     // boxes hold all chunks of their rows; chunks from one head to the next (ta_map)
     int cs, gs;              // bytes in a tile from one 64-value chunk to the next, from 8 rows to the next 8
-    int slots;               // ring slots
+    int k_slots, v_slots;    // slots of the two rings
     int part_rows;           // rows a part in the workspace has room for
     int q_vec, o_vec;        // 16-byte accesses fit q / out
     uint32_t q_flip;         // sign bits to flip (a negative scale)
@@ -117,11 +119,12 @@ struct TaPlan {   // in shared memory
 
 __device__ __forceinline__ long long ta_range_lo(long long total, int ge, int c) { return total * c / ge; }
 
-struct TaSeg {
-    int b, h, rt, kt0, kt1;
-    TaReq r;
+struct TaSeg {       // in shared memory
     long long t0;    // the item's first unit
-    bool head;       // first segment of the CTA
+    int tiles;       // 0: the range has ended
+    int b, h, rt, kt0, nt, L, n, cu0;
+    int head;        // first segment of the CTA
+    int whole;       // all of the item
 };
 
 struct TaIter {
@@ -132,23 +135,27 @@ struct TaIter {
         : u(p.lo), hi(p.hi), base(p.base0), lo(p.lo), b(p.b0) {
         if (u < hi) r = ta_request(A, b, tk);
     }
-    __device__ __forceinline__ bool next(const TaArgs &A, int tk, TaSeg &s) {
-        if (u >= hi) return false;
+    __device__ __forceinline__ void next(const TaArgs &A, int tk, TaSeg &s) {
+        s.tiles = 0;
+        if (u >= hi) return;
         while (u >= base + r.units) {
             base += r.units;
             r = ta_request(A, ++b, tk);
         }
         const long long x = u - base, item = x / r.nt;
         s.b = b;
-        s.r = r;
         s.kt0 = (int)(x - item * r.nt);
-        s.kt1 = (int)min((long long)r.nt, s.kt0 + (hi - u));
+        s.tiles = (int)min((long long)r.nt - s.kt0, hi - u);
         s.h = (int)(item / r.rtn);
         s.rt = (int)(item - (long long)s.h * r.rtn);
+        s.nt = r.nt;
+        s.L = r.L;
+        s.n = r.n;
+        s.cu0 = r.cu0;
         s.t0 = u - s.kt0;
         s.head = u == lo;
-        u += s.kt1 - s.kt0;
-        return true;
+        s.whole = s.tiles == r.nt;
+        u += s.tiles;
     }
 };
 
@@ -311,34 +318,44 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                      const __grid_constant__ TaArgs A) {
     using Lay = TaLayout<NCH, REP>;
     constexpr int TK = Lay::TK, DP = Lay::DP, CH = Lay::CH;
-    constexpr int ROW_WARPS = 4 * CH;
+    constexpr int ROW_WARPS = 4 * CH, K_WARP = ROW_WARPS, MMA_WARP = ROW_WARPS + 1, V_WARP = ROW_WARPS + 2;
     constexpr bool QT = Lay::QT;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *qs = tc_align1024(smem_raw);
-    unsigned char *ring = qs + Lay::Q_BYTES;
-    const int S = A.slots;
-    float *stage = reinterpret_cast<float *>(ring + (size_t)S * Lay::SLOT);   // [128][STAGE_LD] (REP > 1)
-    uint64_t *full = reinterpret_cast<uint64_t *>(ring + (size_t)S * Lay::SLOT + Lay::STAGE);
-    uint64_t *empty = full + S;
-    uint64_t *sfull = empty + S;        // [2] scores in S buffer
+    const int SK = A.k_slots, SV = A.v_slots;
+    unsigned char *kring = qs + Lay::Q_BYTES, *vring = kring + (size_t)SK * Lay::SLOT;
+    float *stage = reinterpret_cast<float *>(vring + (size_t)SV * Lay::SLOT);   // [128][STAGE_LD] (REP > 1)
+    uint64_t *kfull = reinterpret_cast<uint64_t *>(vring + (size_t)SV * Lay::SLOT + Lay::STAGE);
+    uint64_t *kempty = kfull + SK;
+    uint64_t *vfull = kempty + SK;
+    uint64_t *vempty = vfull + SV;
+    uint64_t *sfull = vempty + SV;      // [2] scores in S buffer
     uint64_t *pfull = sfull + 2;        // [2] weights over them (and V ready for use), 4 row warps arrive
     uint64_t *pvdone = pfull + 2;       // [2] the MMAs that read them (and added to O) have completed
     uint64_t *qfull = pvdone + 2;       // [1] Q in place, the row warps arrive
     uint64_t *drain = qfull + 1;
-    long long *wsum = reinterpret_cast<long long *>(drain + 1);   // [10]
-    TaPlan *plan = reinterpret_cast<TaPlan *>(wsum + 10);
+    uint64_t *segfull = drain + 1;      // [TA_RING]
+    TaSeg *segs = reinterpret_cast<TaSeg *>(segfull + TA_RING);   // [TA_RING]
+    TaPlan *plan = reinterpret_cast<TaPlan *>(segs + TA_RING);
     float2 *ml = reinterpret_cast<float2 *>(plan + 1);            // [128] m and l of the replicas / the other group
+    long long *wsum = reinterpret_cast<long long *>(ml);          // [warps], before
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(ml + TA_ROWS);
     uint32_t *wild = tmem_slot + 1;                               // [2 segments][2 words]
-    volatile uint32_t *bad = wild + 4;                            // [TA_BAD] 8-row groups not there
+    volatile uint32_t *more = wild + 4;                           // [1] the rows have another segment
+    volatile uint32_t *bad = wild + 5;                            // [TA_RING] 8-row groups not there
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+        for (int s = 0; s < SK; ++s) {
+            mbar_init(&kfull[s], 1);
+            mbar_init(&kempty[s], 1);
         }
+        for (int s = 0; s < SV; ++s) {
+            mbar_init(&vfull[s], 1);
+            mbar_init(&vempty[s], 1);
+        }
+        for (int s = 0; s < TA_RING; ++s) mbar_init(&segfull[s], 1);
         for (int b = 0; b < 2; ++b) {
             mbar_init(&sfull[b], 1);
             mbar_init(&pfull[b], 4);
@@ -351,7 +368,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         tma_prefetch_desc(&tmap_k);
         tma_prefetch_desc(&tmap_v);
     }
-    if (warp == 1) {
+    if (warp == MMA_WARP) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
@@ -361,81 +378,92 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t *>(tmem_slot);
     const uint64_t deadline = globaltimer() + A.timeout_ns;   // of every wait: one that runs out ends them all
-    TaIter it(A, *plan, TK);
-    TaSeg sg;
 
-    if (warp == 0) {
+    if (warp == K_WARP || warp == V_WARP) {
         // ---------------- K and V tiles ----------------
         // A tile is at most 32 boxes, one a lane: all chunks (fold), or 64-value chunk lane % NCH, of box_rows rows.
-        // The pages of the next tile are looked up while this one's copies are issued; V uses K's.
-        bool dead = false;
-        int k = 0, g = 0;   // ring position, tile counter
+        // The table entries of the next tile are loaded while this one's copies are issued.
+        const bool is_k = warp == K_WARP;
+        const CUtensorMap *map = is_k ? &tmap_k : &tmap_v;
+        uint64_t *full = is_k ? kfull : vfull, *empty = is_k ? kempty : vempty;
+        unsigned char *ring = is_k ? kring : vring;
+        const int S = is_k ? SK : SV;
         const int box = A.box_rows, per = A.fold ? 1 : NCH, p = lane / per, c = lane - p * per;
         const int box_bytes = box * 128 * (A.fold ? NCH : 1);
         const uint32_t dst0 = (uint32_t)((box >> 3) * p * A.gs + c * A.cs);
-        auto page_of = [&](int kt, int &r0) {   // num_blocks: no such page (reads as zeros)
-            const int row = kt * TK + p * box, page = row / A.bs;
-            r0 = row - page * A.bs;
-            if (row >= sg.r.L || page >= A.width || p * box >= TK) return A.num_blocks;
-            const int blk = A.table[(long long)sg.b * A.table_stride + page];
-            return (blk < 0 || blk >= A.num_blocks) ? A.num_blocks : blk;
-        };
-        auto load = [&](const CUtensorMap *map, int boxes, int r0, int blk, int gone) {
-            const int s = k % S;
-            int ok = 1;
-            if (lane == 0) {
-                ok = mbar_wait(&empty[s], ((uint32_t)(k / S) & 1u) ^ 1u, deadline);
-                if (ok) {
-                    if (gone >= 0) bad[g % TA_BAD] = (uint32_t)gone;
-                    mbar_arrive_expect_tx(&full[s], (uint32_t)(boxes * box_bytes));
-                } else {
-                    report(A.status, ST_PIPE_TIMEOUT | 0x210u);
+        bool dead = false;
+        int g = 0, s = 0, seg = 0;   // tiles, ring slot, segments
+        uint32_t phase = 1;          // of the slot's release: the first round finds all slots free
+        TaIter it(A, *plan, TK);
+        while (!dead) {
+            TaSeg *sp = segs + seg % TA_RING;
+            if (is_k) {
+                TaSeg x;
+                it.next(A, TK, x);
+                if (lane == 0) {
+                    *sp = x;
+                    mbar_arrive(&segfull[seg % TA_RING]);
                 }
+                __syncwarp();
+            } else if (!warp_wait(&segfull[seg % TA_RING], (uint32_t)(seg / TA_RING) & 1u, deadline)) {
+                if (lane == 0) report(A.status, ST_PIPE_TIMEOUT | 0x218u);
+                break;
             }
-            if (!__shfl_sync(0xffffffffu, ok, 0)) {
-                dead = true;
-                return;
-            }
-            if (lane < boxes) {
-                unsigned char *dst = ring + (size_t)s * Lay::SLOT + dst0;
-                if (A.fold) tma_load_5d(dst, map, 0, 0, sg.h * A.head_step, r0 >> 3, blk, &full[s]);
-                else tma_load_4d(dst, map, c * 64, r0, sg.h, blk, &full[s]);
-            }
-            ++k;
-        };
-        while (!dead && it.next(A, TK, sg)) {
-            int r0, blk = page_of(sg.kt0, r0), vr0 = 0, vblk = 0, vboxes = 0;
-            for (int kt = sg.kt0; kt <= sg.kt1 && !dead; ++kt) {   // K0, K1 V0, K2 V1, .., V last: the order of use
-                int nr0 = 0, nblk = 0, boxes = 0;
-                if (kt < sg.kt1) {
-                    boxes = (min(max(sg.r.L - kt * TK, 0), TK) + box - 1) / box * per;
-                    // groups of 8 rows whose page is not there
+            const int tiles = sp->tiles, kt0 = sp->kt0, L = sp->L, h = sp->h;
+            if (tiles == 0) break;
+            const int *trow = A.table + (long long)sp->b * A.table_stride;
+            auto entry_of = [&](int kt, int &r0) {   // this lane's table entry; -1: none needed or none there
+                const int row = kt * TK + p * box, page = row / A.bs;
+                r0 = row - page * A.bs;
+                return row < L && page < A.width && p * box < TK ? trow[page] : -1;
+            };
+            int r0, ent = entry_of(kt0, r0);
+            for (int kt = kt0; kt < kt0 + tiles; ++kt, ++g) {
+                const int boxes = (min(max(L - kt * TK, 0), TK) + box - 1) / box * per;
+                const int blk = (ent < 0 || ent >= A.num_blocks) ? A.num_blocks : ent;   // num_blocks reads as zeros
+                const int y0 = r0;
+                if (kt + 1 < kt0 + tiles) ent = entry_of(kt + 1, r0);
+                int ok = 1;
+                if (lane == 0) {
+                    ok = mbar_wait(&empty[s], phase, deadline);
+                    if (!ok) report(A.status, ST_PIPE_TIMEOUT | 0x210u);
+                }
+                if (!__shfl_sync(0xffffffffu, ok, 0)) {
+                    dead = true;
+                    break;
+                }
+                if (is_k) {   // groups of 8 rows whose page is not there
                     const bool none = lane < boxes && blk == A.num_blocks;
-                    const int gone = (int)__reduce_or_sync(
+                    const uint32_t gone = __reduce_or_sync(
                         0xffffffffu, none ? ((1u << (box >> 3)) - 1u) << (p * (box >> 3)) : 0u);
-                    load(&tmap_k, boxes, r0, blk, gone);
-                    ++g;
-                    if (kt + 1 < sg.kt1) nblk = page_of(kt + 1, nr0);
+                    if (lane == 0) bad[g % TA_RING] = gone;
                 }
-                if (kt > sg.kt0 && !dead) load(&tmap_v, vboxes, vr0, vblk, -1);
-                vr0 = r0, vblk = blk, vboxes = boxes;
-                r0 = nr0, blk = nblk;
+                if (lane == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(boxes * box_bytes));
+                __syncwarp();
+                if (lane < boxes) {
+                    unsigned char *dst = ring + (size_t)s * Lay::SLOT + dst0;
+                    if (A.fold) tma_load_5d(dst, map, 0, 0, h * A.head_step, y0 >> 3, blk, &full[s]);
+                    else tma_load_4d(dst, map, c * 64, y0, h, blk, &full[s]);
+                }
+                if (++s == S) s = 0, phase ^= 1u;
             }
+            ++seg;
         }
         if (dead && lane == 0) {   // let the copies already issued land before the shared memory is released
             const uint64_t d2 = globaltimer() + A.timeout_ns;
-            for (int j = (k > S ? k - S : 0); j < k; ++j) mbar_wait(&full[j % S], (uint32_t)(j / S) & 1u, d2);
+            for (int j = (g > S ? g - S : 0); j < g; ++j) mbar_wait(&full[j % S], (uint32_t)(j / S) & 1u, d2);
         }
         __syncwarp();
-    } else if (warp == 1) {
+    } else if (warp == MMA_WARP) {
         // ---------------- MMA issuer ----------------
         // The whole warp runs the loop on warp-uniform values and one elected lane issues: operands stay in uniform
         // registers. (A loop inside `if (lane == 0)` took about 120 cycles an MMA to issue, more than the MMAs.)
         constexpr uint32_t id_s = idesc_f16<T>(TA_ROWS, TK);
         constexpr uint32_t id_o = idesc_f16<T>(TA_ROWS, DP) | (1u << 16);   // B (V) is MN-major
-        const uint32_t tb = __shfl_sync(0xffffffffu, tmem_base, 0), ring0 = smem_u32(ring);
+        const uint32_t tb = __shfl_sync(0xffffffffu, tmem_base, 0), kring0 = smem_u32(kring), vring0 = smem_u32(vring);
         const uint64_t qd = sw128_desc(smem_u32(qs));
-        int k = 0, g = 0, seg = 0;
+        int g = 0, seg = 0, ks = 0, vs = 0;   // tiles, segments, ring slots
+        uint32_t kphase = 0, vphase = 0;
         auto wait = [&](uint64_t *bar, uint32_t parity, unsigned code) {
             if (warp_wait(bar, parity, deadline)) {
                 tc_fence_after();
@@ -444,11 +472,10 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             if (lane == 0) report(A.status, ST_PIPE_TIMEOUT | code);
             return false;
         };
-        auto scores = [&](int gt) {   // S[gt] = Q K^T of the ring's next slot
-            const int s = k % S;
-            if (!wait(&full[s], (uint32_t)(k / S) & 1u, 0x220u)) return false;
+        auto scores = [&](int gt) {   // S[gt] = Q K^T of the next K tile
+            if (!wait(&kfull[ks], kphase, 0x220u)) return false;
             if (gt > 1 && !wait(&pvdone[gt & 1], ((uint32_t)(gt >> 1) & 1u) ^ 1u, 0x228u)) return false;   // P over S
-            const uint64_t kd = ta_k_desc(ring0 + (uint32_t)(s * Lay::SLOT), A.gs);
+            const uint64_t kd = ta_k_desc(kring0 + (uint32_t)(ks * Lay::SLOT), A.gs);
             const uint32_t d = tb + Lay::S_COL + (uint32_t)((gt & 1) * TK);
 #pragma unroll
             for (int i = 0; i < NCH * 4; ++i) {   // 16 values a step; past D both operands hold zeros
@@ -457,39 +484,37 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                 else umma_f16_e(d, qd + (i >> 2) * (TA_ROWS * 128 / 16) + 2 * (i & 3), kdi, id_s, i > 0);
             }
             umma_commit_e(&sfull[gt & 1]);
-            umma_commit_e(&empty[s]);
-            ++k;
+            umma_commit_e(&kempty[ks]);
+            if (++ks == SK) ks = 0, kphase ^= 1u;
             return true;
         };
         bool ok = true;
-        while (ok) {
-            int N = it.next(A, TK, sg) ? sg.kt1 - sg.kt0 : 0;
-            N = __shfl_sync(0xffffffffu, N, 0);
+        while (ok && (ok = wait(&segfull[seg % TA_RING], (uint32_t)(seg / TA_RING) & 1u, 0x238u))) {
+            const int N = __shfl_sync(0xffffffffu, segs[seg % TA_RING].tiles, 0);
             if (N == 0) break;
             ok = wait(qfull, (uint32_t)seg & 1u, 0x230u) && scores(g);
             for (int t = 0; ok && t < N; ++t, ++g) {
                 if (t + 1 < N) ok = scores(g + 1);
                 ok = ok && wait(&pfull[g & 1], (uint32_t)(g >> 1) & 1u, 0x240u);
-                const int s = k % S;
-                ok = ok && wait(&full[s], (uint32_t)(k / S) & 1u, 0x250u);
+                ok = ok && wait(&vfull[vs], vphase, 0x250u);
                 if (!ok) break;
                 const uint32_t o = tb + (CH == 2 ? (uint32_t)((g & 1) * DP) : 0u);
                 const uint32_t p = tb + Lay::S_COL + (uint32_t)((g & 1) * TK);
-                const uint64_t v = ta_v_desc(ring0 + (uint32_t)(s * Lay::SLOT), A.cs, A.gs);
+                const uint64_t v = ta_v_desc(vring0 + (uint32_t)(vs * Lay::SLOT), A.cs, A.gs);
 #pragma unroll
                 for (int i = 0; i < TK / 16; ++i)   // 16 keys a step: 8 columns of P, two groups of rows of V
                     umma_f16_ts_e(o, p + 8 * i, v + (uint64_t)(i * (A.gs >> 3)), id_o, (t >= CH || i > 0) ? 1u : 0u);
                 umma_commit_e(&pvdone[g & 1]);
-                umma_commit_e(&empty[s]);
-                ++k;
+                umma_commit_e(&vempty[vs]);
+                if (++vs == SV) vs = 0, vphase ^= 1u;
             }
             ++seg;
         }
         umma_commit_e(drain);   // every MMA issued has completed once it flips
         warp_wait(drain, 0u, globaltimer() + A.timeout_ns);
-    } else {
+    } else if (warp < ROW_WARPS) {
         // ---------------- rows: softmax and output ----------------
-        const int q4 = warp & 3, grp = CH == 2 ? (warp - 2) >> 2 : 0;
+        const int q4 = warp & 3, grp = warp >> 2;
         const int tid = q4 * 32 + lane;             // lane of tensor memory this thread holds
         constexpr int RR = TA_ROWS / REP, CPT = TK / REP;   // rows; keys of a tile a thread takes
         const int row = tid % RR, part = tid / RR;
@@ -503,35 +528,52 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             }
             tc_fence_after();
         };
-        auto live_rows = [&](const TaSeg &s) { return min(min(s.r.n, A.max_new) * A.G - s.rt * TA_ROWS, TA_ROWS); };
-        auto q_vector = [&](const TaSeg &s, int r, int v) {   // 8 values of row r of the item
-            const int gr = s.rt * TA_ROWS + r, i = gr / A.G, tok = s.r.cu0 + i, d = v * 8;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (d < A.D && tok >= 0 && tok < A.T) {
-                const T *src = reinterpret_cast<const T *>(A.q) + (long long)tok * A.q_t +
-                               (long long)(s.h * A.G + gr - i * A.G) * A.q_h + d;
-                if (A.q_vec) {
-                    x = *reinterpret_cast<const uint4 *>(src);
-                } else {
-                    const uint16_t *e = reinterpret_cast<const uint16_t *>(src);
+        int g = 0, seg = 0;
+        // the next segment, if there is one, and its Q
+        auto open = [&]() {
+            wait(&segfull[seg % TA_RING], (uint32_t)(seg / TA_RING) & 1u, 0x258u);
+            const TaSeg &s = segs[seg % TA_RING];
+            if (threadIdx.x == 0) *more = !dead && s.tiles != 0;   // one thread decides: the warps' barriers must match
+            named_sync(TC_EPI_BAR, 128 * CH);
+            if (!*more) return false;
+            const int live = min(min(s.n, A.max_new) * A.G - s.rt * TA_ROWS, TA_ROWS);
+            const T *q = reinterpret_cast<const T *>(A.q) + (long long)s.cu0 * A.q_t + (long long)s.h * A.G * A.q_h;
+            // row r's values, or NULL for a row that is none
+            auto row_of = [&](int r) -> const T * {
+                const int gr = s.rt * TA_ROWS + r, i = gr / A.G, tok = s.cu0 + i;
+                return r < live && tok >= 0 && tok < A.T ? q + (long long)i * A.q_t + (long long)(gr - i * A.G) * A.q_h
+                                                         : nullptr;
+            };
+            auto vector = [&](const T *src, int d) {   // 8 values
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (src && d < A.D) {
+                    const uint16_t *e = reinterpret_cast<const uint16_t *>(src + d);
                     x = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
                                    e[6] | (uint32_t)e[7] << 16);
                 }
-                x = make_uint4(x.x ^ A.q_flip, x.y ^ A.q_flip, x.z ^ A.q_flip, x.w ^ A.q_flip);
-            }
-            return x;
-        };
-        auto load_q = [&](const TaSeg &s) {
-            const int live = live_rows(s);
-            if constexpr (QT) {   // a thread's own row, 32 columns (64 values) at a time
+                return x;
+            };
+            if constexpr (QT) {   // a thread's own row, 64 values (32 columns) at a time
                 if ((REP > 1 ? 0 : q4 * 32) < live) {
-#pragma unroll 2
+                    const T *src = row_of(row);
+#pragma unroll
                     for (int c = 0; c < NCH; ++c) {
+                        uint4 x[8];
+                        if (A.q_vec) {   // the loads of a chunk in flight together
+#pragma unroll
+                            for (int v = 0; v < 8; ++v)
+                                x[v] = src && c * 64 + v * 8 < A.D
+                                           ? *reinterpret_cast<const uint4 *>(src + c * 64 + v * 8)
+                                           : make_uint4(0, 0, 0, 0);
+                        } else {
+#pragma unroll
+                            for (int v = 0; v < 8; ++v) x[v] = vector(src, c * 64 + v * 8);
+                        }
                         uint32_t w[32];
 #pragma unroll
                         for (int v = 0; v < 8; ++v) {
-                            const uint4 x = row < live ? q_vector(s, row, c * 8 + v) : make_uint4(0, 0, 0, 0);
-                            w[4 * v] = x.x, w[4 * v + 1] = x.y, w[4 * v + 2] = x.z, w[4 * v + 3] = x.w;
+                            w[4 * v] = x[v].x ^ A.q_flip, w[4 * v + 1] = x[v].y ^ A.q_flip;
+                            w[4 * v + 2] = x[v].z ^ A.q_flip, w[4 * v + 3] = x[v].w ^ A.q_flip;
                         }
                         tmem_st32(lane_base + Lay::Q_COL + 32 * c, w);
                     }
@@ -540,56 +582,63 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                 tc_fence_before();
             } else {   // all threads, swizzled as TMA would lay the rows out
                 constexpr int NV = NCH * 8;
-                for (int idx = tid + 128 * grp; idx < live * NV; idx += 128 * CH) {
+#pragma unroll 4
+                for (int idx = threadIdx.x; idx < live * NV; idx += 128 * CH) {
                     const int r = idx / NV, v = idx - r * NV;
-                    *reinterpret_cast<uint4 *>(qs + (v >> 3) * (TA_ROWS * 128) + r * 128 +
-                                               (((v & 7) ^ (r & 7)) << 4)) = q_vector(s, r, v);
+                    const T *src = row_of(r);
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (!A.q_vec) x = vector(src, v * 8);
+                    else if (src && v * 8 < A.D) x = *reinterpret_cast<const uint4 *>(src + v * 8);
+                    *reinterpret_cast<uint4 *>(qs + (v >> 3) * (TA_ROWS * 128) + r * 128 + (((v & 7) ^ (r & 7)) << 4)) =
+                        make_uint4(x.x ^ A.q_flip, x.y ^ A.q_flip, x.z ^ A.q_flip, x.w ^ A.q_flip);
                 }
                 fence_proxy_async();
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(qfull);
+            return true;
         };
-        int g = 0, kbase = 0, seg = 0;
-        bool has = it.next(A, TK, sg);
-        if (threadIdx.x == TC_EPI_LEAD) A.desc[blockIdx.x].split = 0;
-        if (has) {
-            if (threadIdx.x == TC_EPI_LEAD && sg.kt0 > 0) {
+        bool has = open();
+        if (threadIdx.x == 0) {
+            A.desc[blockIdx.x].split = 0;
+            if (has && segs[0].kt0 > 0) {
+                const TaSeg &x = segs[0];
                 TaDesc d;
-                d.t0 = sg.t0;
+                d.t0 = x.t0;
                 d.total = plan->total;
-                d.split = sg.t0 >= ta_range_lo(plan->total, plan->ge, blockIdx.x - 1);
-                d.nt = sg.r.nt;
+                d.split = x.t0 >= ta_range_lo(plan->total, plan->ge, blockIdx.x - 1);
+                d.nt = x.nt;
                 d.ge = plan->ge;
-                d.cu0 = sg.r.cu0;
-                d.n = sg.r.n;
-                d.h = sg.h;
-                d.rt = sg.rt;
+                d.cu0 = x.cu0;
+                d.n = x.n;
+                d.h = x.h;
+                d.rt = x.rt;
                 d.pad = 0;
                 A.desc[blockIdx.x] = d;
             }
-            load_q(sg);
         }
         while (has) {
-            const int ctx = sg.r.L - sg.r.n, N = sg.kt1 - sg.kt0, live = live_rows(sg), g0 = g;
-            const int gr = sg.rt * TA_ROWS + row, tok_i = gr / A.G, tok = sg.r.cu0 + tok_i;
+            const TaSeg &sg = segs[seg % TA_RING];
+            const int N = sg.tiles, L = sg.L, ctx = L - sg.n, kt0 = sg.kt0, g0 = g;
+            const int live = min(min(sg.n, A.max_new) * A.G - sg.rt * TA_ROWS, TA_ROWS);
+            const int gr = sg.rt * TA_ROWS + row, tok_i = gr / A.G, tok = sg.cu0 + tok_i;
             const bool mine = row < live && tok >= 0 && tok < A.T;
             const bool warp_live = (REP > 1 ? 0 : q4 * 32) < live;
             unsigned long long see = 0;
             if (mine) {
                 see = A.mask ? (unsigned long long)A.mask[tok] : (2ull << tok_i) - 1ull;
-                if (sg.r.n < 64) see &= (1ull << sg.r.n) - 1ull;
+                if (sg.n < 64) see &= (1ull << sg.n) - 1ull;
             }
             float m = -INFINITY, l = 0.0f;
             for (int t = 0; t < N; ++t, ++g) {
                 const int buf = g & 1;
                 if (CH == 2 && buf != grp) continue;
-                const int k0 = (sg.kt0 + t) * TK;
+                const int k0 = (kt0 + t) * TK;
                 const uint32_t use = (uint32_t)(g >> 1);
                 const bool past = k0 + TK > ctx;
                 const uint32_t s_col = lane_base + Lay::S_COL + (uint32_t)(buf * TK);
                 wait(&sfull[buf], use & 1u, 0x260u);
-                const uint32_t gone = bad[g % TA_BAD];
+                const uint32_t gone = bad[g % TA_RING];
                 if (warp_live) {
                     // W keys at a time; a thread with more (CH = 2, whose ten warps leave it 168 registers) reads its
                     // scores twice
@@ -673,14 +722,14 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                 }
                 if (past) {
                     // rows of V that not every row sees: zeros past the length, no infinities or NaN before it
-                    const int vi = kbase + (t + 1 < N ? 2 * t + 2 : 2 * N - 1), r0 = max(ctx - k0, 0);
-                    wait(&full[vi % S], (uint32_t)(vi / S) & 1u, 0x290u);
-                    unsigned char *vs = ring + (size_t)(vi % S) * Lay::SLOT;
+                    const int r0 = max(ctx - k0, 0);
+                    wait(&vfull[g % SV], (uint32_t)(g / SV) & 1u, 0x290u);
+                    unsigned char *vs = vring + (size_t)(g % SV) * Lay::SLOT;
                     for (int idx = tid; idx < (TK - r0) * NCH * 8 && !dead; idx += 128) {
                         const int r = r0 + idx / (NCH * 8), v = idx % (NCH * 8), j = k0 + r;
                         uint4 *p = reinterpret_cast<uint4 *>(vs + (r >> 3) * A.gs + (v >> 3) * A.cs + (r & 7) * 128 +
                                                              (((v & 7) ^ (r & 7)) << 4));
-                        if (j >= sg.r.L) {
+                        if (j >= L) {
                             *p = make_uint4(0, 0, 0, 0);
                             continue;
                         }
@@ -706,15 +755,13 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             }
             // the next item's Q may go in once this one's last scores are done
             if (CH == 2) wait(&sfull[(g - 1) & 1], (uint32_t)((g - 1) >> 1) & 1u, 0x298u);
-            kbase += 2 * N;
-            const TaSeg cur = sg;
-            has = it.next(A, TK, sg);
-            if (has) load_q(sg);
+            ++seg;
+            has = open();
             wait(&pvdone[(g - 1) & 1], (uint32_t)((g - 1) >> 1) & 1u, 0x2a0u);
             if (CH == 2 && N > 1) wait(&pvdone[g & 1], (uint32_t)((g - 2) >> 1) & 1u, 0x2a8u);
-            if (threadIdx.x == TC_EPI_LEAD) {
-                wild[((seg & 1) ^ 1) * 2] = 0;
-                wild[((seg & 1) ^ 1) * 2 + 1] = 0;
+            if (threadIdx.x == 0) {   // the words of the segment after this one
+                wild[(seg & 1) * 2] = 0;
+                wild[(seg & 1) * 2 + 1] = 0;
             }
             // join the replicas' or the two groups' sums: a factor for each, and the common m and l
             float f0 = 1.0f, f1 = 0.0f;
@@ -751,24 +798,24 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             } else {
                 named_sync(TC_EPI_BAR, 128);
             }
-            const volatile uint32_t *wv = wild + (seg & 1) * 2;
+            const volatile uint32_t *wv = wild + ((seg & 1) ^ 1) * 2;
             const unsigned long long wn = see & (wv[0] | (unsigned long long)wv[1] << 32);
-            const bool whole = cur.kt0 == 0 && cur.kt1 == cur.r.nt;
+            const bool whole = sg.whole;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const size_t prow = (size_t)(2 * blockIdx.x + (cur.head ? 0 : 1)) * A.part_rows + row;
+            const size_t prow = (size_t)(2 * blockIdx.x + (sg.head ? 0 : 1)) * A.part_rows + row;
             T *dst = reinterpret_cast<T *>(A.out) + (long long)tok * A.o_t +
-                     (long long)(cur.h * A.G + gr - tok_i * A.G) * A.o_h;
+                     (long long)(sg.h * A.G + gr - tok_i * A.G) * A.o_h;
             // NV values of the row from column c: the parts go to the workspace in 32 bits, a whole item's to the output
             auto put = [&](auto &o, int c) {
                 constexpr int NV = sizeof(o) / sizeof(float);
                 if (wn) {   // the values taken out above, for the rows that see them
                     for (unsigned long long left = wn; left; left &= left - 1) {
                         const int j = ctx + __ffsll((long long)left) - 1, page = j / A.bs;
-                        if (j < cur.kt0 * TK || j >= cur.kt1 * TK || page >= A.width) continue;
-                        const int blk = A.table[(long long)cur.b * A.table_stride + page];
+                        if (j < kt0 * TK || j >= (kt0 + N) * TK || page >= A.width) continue;
+                        const int blk = A.table[(long long)sg.b * A.table_stride + page];
                         if (blk < 0 || blk >= A.num_blocks) continue;
                         const T *v = reinterpret_cast<const T *>(A.v) + blk * A.v_b + (j - page * A.bs) * A.v_r +
-                                     cur.h * A.v_h;
+                                     sg.h * A.v_h;
 #pragma unroll
                         for (int e = 0; e < NV; ++e) {
                             if (c + e >= A.D) break;
@@ -851,13 +898,12 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             }
             tc_fence_before();
             if (CH == 2) named_sync(TC_EPI_BAR, 256);   // both groups have read both O
-            ++seg;
         }
     }
     // all roles done: free TMEM after every TMEM access and MMA of the CTA has completed
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
+    if (warp == MMA_WARP) {
         tc_fence_after();
         tmem_dealloc(tmem_base, 512);
     }
@@ -987,7 +1033,8 @@ static int launch_ta(const CUtensorMap &mk, const CUtensorMap &mv, TaArgs A, cud
     int slots = (max_smem_optin(dev) - fixed) / Lay::SLOT;
     if (slots > 12) slots = 12;
     if (slots < 4) return VT_EARG;
-    A.slots = slots;
+    A.k_slots = (slots + 1) / 2;
+    A.v_slots = slots / 2;
     A.cs = A.fold ? 1024 : Lay::TK * 128;
     A.gs = A.fold ? NCH * 1024 : 1024;
     const int smem = fixed + slots * Lay::SLOT;
