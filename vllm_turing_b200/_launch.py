@@ -1,15 +1,21 @@
-"""Launches a C entry on the device its tensors live on, on that device's current stream."""
+"""Launches a C entry on the device its tensors live on, on that device's current stream, and the refusals the entries
+share. The calls below run once per layer of a decode step, so what every call does is kept to a few plain comparisons;
+a refused call explains itself on its own path."""
 import torch
 
+# the current device and stream without building Python objects for them (2 x 3 us a call otherwise)
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_stream = (getattr(torch._C, "_cuda_getCurrentRawStream", None)
+           or (lambda i: torch.cuda.current_stream(i).cuda_stream))
 
-def launch(name, fn, device, *args):
-    """fn(*args, stream) with `device` current; raises on a non-zero status."""
-    i = device.index
-    if i == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+
+def launch(name, fn, index, *args):
+    """fn(*args, stream) with device `index` current; raises on a non-zero status."""
+    if index == _device():
+        rc = fn(*args, _stream(index))
     else:
-        with torch.cuda.device(i):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(index))
     if rc != 0:
         raise RuntimeError(f"{name} failed: {rc}")
 
@@ -19,23 +25,15 @@ def need(ok, what):
         raise ValueError(what)
 
 
-def same_device(what, *tensors):
-    """Every given tensor is a CUDA tensor of the first one's device."""
-    d = tensors[0].device
-    if d.type != "cuda" or any(t is not None and t.device != d for t in tensors):
-        raise ValueError(f"{what}: CUDA tensors of one device are needed, got "
-                         f"{[str(t.device) for t in tensors if t is not None]}")
-    return d
+def refuse_devices(what, *tensors):
+    raise ValueError(f"{what}: CUDA tensors of one device are needed, got "
+                     f"{[str(t.device) for t in tensors if t is not None]}")
 
 
-def dtype_code(what, t, *others):
-    """0 fp16 / 1 bf16, the same for every given tensor."""
-    if t.dtype not in (torch.float16, torch.bfloat16) or any(o is not None and o.dtype != t.dtype for o in others):
-        raise TypeError(f"{what}: one dtype, float16 or bfloat16, got "
-                        f"{[str(x.dtype) for x in (t, *others) if x is not None]}")
-    return 0 if t.dtype == torch.float16 else 1
+def refuse_dtypes(what, *tensors):
+    raise TypeError(f"{what}: one dtype, float16 or bfloat16, got {[str(t.dtype) for t in tensors if t is not None]}")
 
 
 def vector(t, dtype, n):
     """A contiguous 1-D tensor of n elements."""
-    return t.dtype == dtype and t.dim() == 1 and t.shape[0] == n and t.is_contiguous()
+    return t.dtype == dtype and t.shape == (n,) and t.is_contiguous()

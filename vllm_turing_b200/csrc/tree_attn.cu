@@ -47,9 +47,7 @@ namespace vt {
 
 constexpr int TA_MAX_NEW = 64;
 constexpr int TA_ROWS = 128;
-constexpr int TA_BARS = 3072;        // barriers and small shared state, bytes
-constexpr int TA_RING = 16;          // entries of the rings of segments and of "pages that are not there" words: more
-                                     // than the tiles between the K warp and the rows (at most 6 slots + 4)
+constexpr int TA_BARS = 2048;        // barriers and small shared state, bytes
 constexpr float TA_RAISE = 8.0f;     // log2 of the factor by which weights may pass the running maximum
 
 template <int NCH, int REP> struct TaLayout {        // NCH: 64-value chunks of the head
@@ -62,6 +60,9 @@ template <int NCH, int REP> struct TaLayout {        // NCH: 64-value chunks of 
     static constexpr int STAGE_LD = 33;                            // floats a row of the staging area
     static constexpr int STAGE = REP > 1 ? (TA_ROWS * STAGE_LD * 4 + 1023) / 1024 * 1024 : 0;
     static constexpr int SLOT = NCH * TK * 128;
+    // entries of the rings of segments and of "pages that are not there" words: more than the K ring's slots (half of
+    // the 7 that fit, or of 12) + 2, which is how far the K warp can be ahead of the rows
+    static constexpr int RING = SLOT >= 32768 ? 8 : 16;
     static constexpr int S_COL = CH * DP, Q_COL = S_COL + 2 * TK;  // tensor memory: O (O0 O1) | S0 S1 (P over S) | Q
     static_assert(Q_COL + (QT ? DP / 2 : 0) <= 512, "tensor memory");
 };
@@ -320,6 +321,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
     constexpr int TK = Lay::TK, DP = Lay::DP, CH = Lay::CH;
     constexpr int ROW_WARPS = 4 * CH, K_WARP = ROW_WARPS, MMA_WARP = ROW_WARPS + 1, V_WARP = ROW_WARPS + 2;
     constexpr bool QT = Lay::QT;
+    constexpr int TA_RING = Lay::RING;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *qs = tc_align1024(smem_raw);
     const int SK = A.k_slots, SV = A.v_slots;
@@ -909,86 +911,104 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
     }
 }
 
-// Joins the parts of the items that a range boundary cuts: block (c - 1, chunk of rows) for the item that CTA c's
-// range starts inside of, when c is the first such CTA. Contributors are CTAs c - 1 .. c1 in order; WPR warps share a
-// row's contributors and add up in warp order.
-constexpr int TJ_THREADS = 512;
-template <typename T, int NCH, int WPR>
-__global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_constant__ TaArgs A) {
-    constexpr int DP = NCH * 64, RPB = TJ_THREADS / 32 / WPR, E = DP / 32;
-    __shared__ float acc_sm[RPB][WPR > 1 ? WPR - 1 : 1][DP];
-    __shared__ float l_sm[RPB][WPR];
+// Joins the parts of the items that a range boundary cuts. Each block reads which CTAs start inside an item, as the
+// first to do so (desc.split), and lists them; the blocks then share out the (item, row) pairs, a row a group of WPR
+// warps: all 8 warps of the block where there are few rows (one token over a long context is cut into many parts), one
+// warp where there are many. A row's contributors are the CTAs c - 1 .. c1 in order; the warps' sums add up in warp
+// order.
+constexpr int TJ_THREADS = 256, TJ_WARPS = TJ_THREADS / 32;
+template <typename T, int NCH>
+__global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_constant__ TaArgs A, int ctas) {
+    constexpr int DP = NCH * 64, E = DP / 32;
+    __shared__ float acc_sm[TJ_WARPS - 1][DP];
+    __shared__ float l_sm[TJ_WARPS];
+    __shared__ short list[TJ_THREADS];
+    __shared__ int found[TJ_WARPS];
     pdl_launch_dependents();
     pdl_wait();
-    const int c = blockIdx.x + 1;
-    const TaDesc d = A.desc[c];
-    if (!d.split) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rb = warp / WPR, wr = warp % WPR;
-    const int r = blockIdx.y * RPB + rb;
-    const int gr = d.rt * TA_ROWS + r, i = gr / A.G, tok = d.cu0 + i;
-    const bool mine = r < min(min(d.n, A.max_new) * A.G - d.rt * TA_ROWS, TA_ROWS) && tok >= 0 && tok < A.T;
-    const int first = (d.t0 == ta_range_lo(d.total, d.ge, c - 1)) ? 2 * (c - 1) : 2 * (c - 1) + 1;
-    int c1 = (int)((d.t0 + d.nt - 1) * d.ge / d.total);   // the CTA holding the item's last unit
-    while (c1 + 1 < d.ge && ta_range_lo(d.total, d.ge, c1 + 1) <= d.t0 + d.nt - 1) ++c1;
-    const int nc = c1 - (c - 1) + 1;
-    auto slot = [&](int j) { return (size_t)(j == 0 ? first : 2 * (c - 1 + j)) * A.part_rows + r; };
-    float M = -INFINITY;
-    if (mine)
-        for (int j = lane; j < nc; j += 32) M = fmaxf(M, A.stats[slot(j)].x);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // up to TJ_THREADS cut items at a time (one pass, unless the GPU has more SMs than that)
+    for (int base = 0; base < ctas; base += TJ_THREADS) {
+        const bool cut = base + tid < ctas && A.desc[base + tid].split != 0;
+        const unsigned bal = __ballot_sync(0xffffffffu, cut);
+        if (lane == 0) found[warp] = __popc(bal);
+        __syncthreads();
+        int at = __popc(bal & ((1u << lane) - 1u)), items = 0;
+        for (int w = 0; w < TJ_WARPS; ++w) {
+            if (w < warp) at += found[w];
+            items += found[w];
+        }
+        if (cut) list[at] = (short)tid;
+        __syncthreads();
+        const int rows = A.part_rows, wpr = items * rows <= 4 * (int)gridDim.x ? TJ_WARPS : 1;
+        const int groups = TJ_WARPS / wpr, wr = wpr > 1 ? warp : 0;
+        for (int w0 = blockIdx.x * groups; w0 < items * rows; w0 += gridDim.x * groups) {
+            const int task = w0 + (wpr > 1 ? 0 : warp), item = task / rows, r = task - item * rows;
+            const bool some = task < items * rows;
+            const int c = base + list[some ? item : 0];
+            const TaDesc d = A.desc[c];
+            const int gr = d.rt * TA_ROWS + r, i = gr / A.G, tok = d.cu0 + i;
+            const bool mine = some && r < min(min(d.n, A.max_new) * A.G - d.rt * TA_ROWS, TA_ROWS) && tok >= 0 && tok < A.T;
+            float acc[E], l = 0.0f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if (M == -INFINITY) M = 0.0f;
-    float acc[E], l = 0.0f;
+            for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+            if (mine) {
+                const int first = d.t0 == ta_range_lo(d.total, d.ge, c - 1) ? 2 * (c - 1) : 2 * (c - 1) + 1;
+                const long long last = d.t0 + d.nt - 1;
+                int c1 = (int)(last * d.ge / d.total);   // the CTA holding the item's last unit
+                while (c1 + 1 < d.ge && ta_range_lo(d.total, d.ge, c1 + 1) <= last) ++c1;
+                const int nc = c1 - (c - 1) + 1;
+                auto slot = [&](int j) { return (size_t)(j == 0 ? first : 2 * (c - 1 + j)) * rows + r; };
+                float M = -INFINITY;
+                for (int j = lane; j < nc; j += 32) M = fmaxf(M, A.stats[slot(j)].x);
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    if (mine) {
+                for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+                if (M == -INFINITY) M = 0.0f;
 #pragma unroll 4
-        for (int j = wr; j < nc; j += WPR) {
-            const size_t s = slot(j);
-            const float2 st = A.stats[s];
-            const float w = ta_exp2(st.x - M);
-            l += w * st.y;
-            const float2 *p = reinterpret_cast<const float2 *>(A.parts + s * DP);
+                for (int j = wr; j < nc; j += wpr) {
+                    const size_t s = slot(j);
+                    const float2 st = A.stats[s];
+                    float2 v[E / 2];
+                    const float2 *p = reinterpret_cast<const float2 *>(A.parts + s * DP);
 #pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                const float2 v = p[lane + 16 * e];
-                if (w != 0.0f) {
-                    acc[e] = __fmaf_rn(w, v.x, acc[e]);
-                    acc[e + 1] = __fmaf_rn(w, v.y, acc[e + 1]);
+                    for (int e = 0; e < E / 2; ++e) v[e] = p[lane + 32 * e];
+                    const float w = ta_exp2(st.x - M);
+                    l += w * st.y;
+#pragma unroll
+                    for (int e = 0; e < E / 2; ++e) {   // a part without keys may hold anything
+                        acc[2 * e] = w != 0.0f ? __fmaf_rn(w, v[e].x, acc[2 * e]) : acc[2 * e];
+                        acc[2 * e + 1] = w != 0.0f ? __fmaf_rn(w, v[e].y, acc[2 * e + 1]) : acc[2 * e + 1];
+                    }
                 }
             }
-        }
-    }
-    if (WPR > 1) {
-        if (wr > 0) {
+            if (wpr > 1) {
+                if (wr > 0) {
 #pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                acc_sm[rb][wr - 1][2 * lane + 32 * e] = acc[e];
-                acc_sm[rb][wr - 1][2 * lane + 32 * e + 1] = acc[e + 1];
+                    for (int e = 0; e < E; ++e) acc_sm[wr - 1][32 * e + lane] = acc[e];
+                }
+                if (lane == 0) l_sm[wr] = l;
+                __syncthreads();
+                if (wr == 0) {
+                    for (int w = 1; w < wpr; ++w) {
+                        l += l_sm[w];
+#pragma unroll
+                        for (int e = 0; e < E; ++e) acc[e] += acc_sm[w - 1][32 * e + lane];
+                    }
+                }
+                __syncthreads();
+            }
+            if (!mine || wr > 0) continue;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            T *dst = reinterpret_cast<T *>(A.out) + (long long)tok * A.o_t + (long long)(d.h * A.G + gr - i * A.G) * A.o_h;
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) {
+                const int col = 2 * (lane + 32 * e);
+                if (col >= A.D) continue;
+                dst[col] = f2t<T>(acc[2 * e] * inv);
+                dst[col + 1] = f2t<T>(acc[2 * e + 1] * inv);
             }
         }
-        if (lane == 0) l_sm[rb][wr] = l;
         __syncthreads();
-        if (wr > 0) return;
-#pragma unroll
-        for (int w = 1; w < WPR; ++w) {
-            l += l_sm[rb][w];
-#pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                acc[e] += acc_sm[rb][w - 1][2 * lane + 32 * e];
-                acc[e + 1] += acc_sm[rb][w - 1][2 * lane + 32 * e + 1];
-            }
-        }
-    }
-    if (!mine) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T *dst = reinterpret_cast<T *>(A.out) + (long long)tok * A.o_t + (long long)(d.h * A.G + gr - i * A.G) * A.o_h;
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-        const int col = 2 * lane + 32 * e;
-        if (col >= A.D) continue;
-        dst[col] = f2t<T>(acc[e] * inv);
-        dst[col + 1] = f2t<T>(acc[e + 1] * inv);
     }
 }
 
@@ -1049,11 +1069,7 @@ static int launch_ta(const CUtensorMap &mk, const CUtensorMap &mv, TaArgs A, cud
     if (int rc = launch_k(tree_attn_kernel<T, NCH, REP>, dim3(grid), dim3(Lay::THREADS), smem, s, true, mk, mv, A))
         return rc;
     if (grid < 2) return 0;
-    if (A.part_rows <= 32)
-        return launch_k(tree_join_kernel<T, NCH, 4>, dim3(grid - 1, (A.part_rows + 3) / 4), dim3(TJ_THREADS), 0, s, true,
-                        A);
-    return launch_k(tree_join_kernel<T, NCH, 1>, dim3(grid - 1, (A.part_rows + 15) / 16), dim3(TJ_THREADS), 0, s, true,
-                    A);
+    return launch_k(tree_join_kernel<T, NCH>, dim3(2 * grid), dim3(TJ_THREADS), 0, s, true, A, grid);
 }
 
 template <typename T, int NCH>

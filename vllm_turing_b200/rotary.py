@@ -11,7 +11,7 @@ from typing import NamedTuple
 import torch
 
 from . import _build
-from ._launch import dtype_code, launch, need, same_device, vector
+from ._launch import launch, need, refuse_devices, refuse_dtypes, vector
 
 SCALINGS = ("none", "linear", "ntk", "yarn", "llama3")
 MAX_ROT = 1024
@@ -67,17 +67,25 @@ def rope_frequencies(rot_dim, base=10000.0, scaling="none", factor=1.0, original
     return RopeFreqs(turns, scale, rot_dim)
 
 
-def _heads(what, x, T, D):
-    need(x.dim() == 3 and x.shape[0] == T and x.shape[2] == D and (x.stride(2) == 1 or x.numel() == 0 or D == 1),
-         f"{what}: [T, heads, D] with a contiguous last dimension, T = {T}, D = {D}, got {tuple(x.shape)} "
-         f"strides {x.stride()}")
+_STRIDES8, _STRIDES14 = ctypes.c_longlong * 8, ctypes.c_longlong * 14
+_CODE = {torch.float16: 0, torch.bfloat16: 1}
 
 
-def _freq_checks(what, freqs, D, positions, T):
-    need(isinstance(freqs, RopeFreqs) and vector(freqs.turns, torch.float64, freqs.rot_dim // 2),
-         f"{what}: freqs must come from rope_frequencies")
+def _heads(what, x, shape):
+    need(x.shape == shape and (x.stride(2) == 1 or x.numel() == 0 or shape[2] == 1),
+         f"{what} must be {list(shape)} with a contiguous last dimension, got {list(x.shape)} strides {x.stride()}")
+
+
+def _refuse_freqs(what, freqs, positions, T, D):
+    need(isinstance(freqs, RopeFreqs) and freqs.turns.dim() == 1
+         and vector(freqs.turns, torch.float64, freqs.rot_dim // 2), f"{what}: freqs must come from rope_frequencies")
     need(freqs.rot_dim <= D, f"{what}: rotates {freqs.rot_dim} of {D} values")
     need(vector(positions, torch.int64, T), f"{what}: positions must be contiguous int64 [T]")
+
+
+def _plain(x, shape):
+    """[T, heads, D] as given, with its values side by side (what the kernel reads without looking further)."""
+    return x.shape == shape and x.stride()[2] == 1
 
 
 def rotary(q, k, positions, freqs, interleaved=False, transpose=False, q_out=None, k_out=None):
@@ -86,33 +94,47 @@ def rotary(q, k, positions, freqs, interleaved=False, transpose=False, q_out=Non
     given; they may be q and k themselves. transpose applies the transposed map: the gradient with respect to the input,
     given the gradient of the output (and, for factor 1, the rotation back)."""
     need(q is not None and q.dim() == 3, "rotary: q must be [T, heads, D]")
-    T, Hq, D = q.shape
-    _heads("rotary q", q, T, D)
-    if k is not None:
-        _heads("rotary k", k, T, D)
-    _freq_checks("rotary", freqs, D, positions, T)
+    qshape = q.shape
+    T, Hq, D = qshape
     if q_out is None:
         q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
-    if k is not None and k_out is None:
-        k_out = torch.empty(T, k.shape[1], D, dtype=k.dtype, device=k.device)
-    need(q_out.shape == q.shape and (k is None or k_out.shape == k.shape), "rotary: outputs have the inputs' shapes")
-    _heads("rotary q_out", q_out, T, D)
+    if not (_plain(q, qshape) and _plain(q_out, qshape)):
+        _heads("rotary: q", q, qshape)
+        _heads("rotary: q_out", q_out, qshape)
+    Hkv = 0
     if k is not None:
-        _heads("rotary k_out", k_out, T, D)
+        Hkv = k.shape[1] if k.dim() == 3 else -1
+        kshape = (T, Hkv, D)
+        need(Hkv >= 0, "rotary: k must be [T, heads, D]")
+        if k_out is None:
+            k_out = torch.empty(T, Hkv, D, dtype=k.dtype, device=k.device)
+        if not (_plain(k, kshape) and _plain(k_out, kshape)):
+            _heads("rotary: k", k, kshape)
+            _heads("rotary: k_out", k_out, kshape)
     else:
         k_out = None
-    code = dtype_code("rotary", q, k, q_out, k_out)
-    dev = same_device("rotary", q, k, positions, freqs.turns, q_out, k_out)
-    Hkv = k.shape[1] if k is not None else 0
+    if not (isinstance(freqs, RopeFreqs) and freqs.rot_dim <= D and vector(positions, torch.int64, T)
+            and vector(freqs.turns, torch.float64, freqs.rot_dim // 2)):
+        _refuse_freqs("rotary", freqs, positions, T, D)
+    dt, dev = q.dtype, q.device
+    code = _CODE.get(dt)
+    if code is None or q_out.dtype != dt or (k is not None and (k.dtype != dt or k_out.dtype != dt)):
+        refuse_dtypes("rotary", q, k, q_out, k_out)
+    if not (dev.type == "cuda" and positions.device == dev and freqs.turns.device == dev and q_out.device == dev
+            and (k is None or (k.device == dev and k_out.device == dev))):
+        refuse_devices("rotary", q, k, positions, freqs.turns, q_out, k_out)
     if T == 0 or Hq + Hkv == 0 or D == 0:
         return q_out, k_out
-    ks, ko = (k.stride(), k_out.stride()) if k is not None else ((0, 0), (0, 0))
     qs, qo = q.stride(), q_out.stride()
-    strides = (ctypes.c_longlong * 8)(qs[0], qs[1], qo[0], qo[1], ks[0], ks[1], ko[0], ko[1])
-    launch("vt_rotary", _build.load().vt_rotary, dev, q.data_ptr(), q_out.data_ptr(),
-           k.data_ptr() if k is not None else None, k_out.data_ptr() if k is not None else None, strides,
-           positions.data_ptr(), freqs.turns.data_ptr(), freqs.factor, int(interleaved), int(transpose), T, Hq, Hkv, D,
-           freqs.rot_dim, code)
+    if k is not None:
+        ks, ko = k.stride(), k_out.stride()
+        strides = _STRIDES8(qs[0], qs[1], qo[0], qo[1], ks[0], ks[1], ko[0], ko[1])
+    else:
+        strides = _STRIDES8(qs[0], qs[1], qo[0], qo[1])
+    launch("vt_rotary", _build.load().vt_rotary, dev.index, q.data_ptr(), q_out.data_ptr(),
+           None if k is None else k.data_ptr(), None if k is None else k_out.data_ptr(), strides,
+           positions.data_ptr(), freqs.turns.data_ptr(), freqs.factor, bool(interleaved), bool(transpose), T, Hq, Hkv,
+           D, freqs.rot_dim, code)
     return q_out, k_out
 
 
@@ -120,34 +142,47 @@ def rotary_cache(q, k, v, positions, slots, k_cache, v_cache, freqs, interleaved
     """q_out: q [T, Hq, D] rotated as by rotary(); k [T, Hkv, D] rotated and v [T, Hkv, D] go to rows slots (int64 [T])
     of the paged cache k_cache, v_cache [num_blocks, block_size, Hkv, D] (any strides, last dimension contiguous). A
     token whose slot is outside the cache (step_tables gives -1) writes no k and v. Slots inside it must differ."""
-    need(q is not None and q.dim() == 3, "rotary_cache: q must be [T, heads, D]")
-    T, Hq, D = q.shape
-    _heads("rotary_cache q", q, T, D)
-    _heads("rotary_cache k", k, T, D)
-    _heads("rotary_cache v", v, T, D)
+    need(q is not None and q.dim() == 3 and k.dim() == 3, "rotary_cache: q and k must be [T, heads, D]")
+    qshape = q.shape
+    T, Hq, D = qshape
     Hkv = k.shape[1]
-    need(Hkv >= 1 and v.shape == k.shape, "rotary_cache: k and v must be [T, Hkv, D] alike, Hkv >= 1")
-    need(k_cache.dim() == 4 and v_cache.shape == k_cache.shape and k_cache.shape[1] >= 1
-         and tuple(k_cache.shape[2:]) == (Hkv, D) and (k_cache.numel() == 0 or (k_cache.stride(3) == 1
-                                                                               and v_cache.stride(3) == 1)),
-         f"rotary_cache: the caches must be [num_blocks, block_size, {Hkv}, {D}] with a contiguous last dimension")
-    _freq_checks("rotary_cache", freqs, D, positions, T)
-    need(vector(slots, torch.int64, T), "rotary_cache: slots must be contiguous int64 [T]")
+    kshape = (T, Hkv, D)
     if q_out is None:
         q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
-    need(q_out.shape == q.shape, "rotary_cache: q_out has q's shape")
-    _heads("rotary_cache q_out", q_out, T, D)
-    code = dtype_code("rotary_cache", q, k, v, k_cache, v_cache, q_out)
-    dev = same_device("rotary_cache", q, k, v, positions, slots, k_cache, v_cache, freqs.turns, q_out)
+    if not (_plain(q, qshape) and _plain(q_out, qshape) and _plain(k, kshape) and _plain(v, kshape) and Hkv >= 1):
+        _heads("rotary_cache: q", q, qshape)
+        _heads("rotary_cache: q_out", q_out, qshape)
+        _heads("rotary_cache: k", k, kshape)
+        _heads("rotary_cache: v", v, kshape)
+        need(Hkv >= 1, "rotary_cache: k and v must have a head")
+    cshape, kc, vc = k_cache.shape, k_cache.stride(), v_cache.stride()
+    if not (len(cshape) == 4 and v_cache.shape == cshape and cshape[1] >= 1 and cshape[2] == Hkv and cshape[3] == D
+            and ((kc[3] == 1 and vc[3] == 1) or k_cache.numel() == 0)):
+        raise ValueError(f"rotary_cache: the caches must be [num_blocks, block_size, {Hkv}, {D}] with a contiguous "
+                         f"last dimension, got {list(cshape)} and {list(v_cache.shape)}")
+    if not (isinstance(freqs, RopeFreqs) and freqs.rot_dim <= D and vector(positions, torch.int64, T)
+            and vector(freqs.turns, torch.float64, freqs.rot_dim // 2)):
+        _refuse_freqs("rotary_cache", freqs, positions, T, D)
+    if not vector(slots, torch.int64, T):
+        raise ValueError("rotary_cache: slots must be contiguous int64 [T]")
+    dt, dev = q.dtype, q.device
+    code = _CODE.get(dt)
+    if code is None or not (k.dtype == dt and v.dtype == dt and q_out.dtype == dt and k_cache.dtype == dt
+                            and v_cache.dtype == dt):
+        refuse_dtypes("rotary_cache", q, k, v, k_cache, v_cache, q_out)
+    if not (dev.type == "cuda" and k.device == dev and v.device == dev and positions.device == dev
+            and slots.device == dev and k_cache.device == dev and v_cache.device == dev and freqs.turns.device == dev
+            and q_out.device == dev):
+        refuse_devices("rotary_cache", q, k, v, positions, slots, k_cache, v_cache, freqs.turns, q_out)
     if T == 0 or D == 0:
         return q_out
-    qs, qo, ks, vs, kc, vc = q.stride(), q_out.stride(), k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
-    strides = (ctypes.c_longlong * 14)(qs[0], qs[1], qo[0], qo[1], ks[0], ks[1], vs[0], vs[1], kc[0], kc[1], kc[2],
-                                       vc[0], vc[1], vc[2])
-    launch("vt_rotary_cache", _build.load().vt_rotary_cache, dev, q.data_ptr(), q_out.data_ptr(), k.data_ptr(),
+    qs, qo, ks, vs = q.stride(), q_out.stride(), k.stride(), v.stride()
+    strides = _STRIDES14(qs[0], qs[1], qo[0], qo[1], ks[0], ks[1], vs[0], vs[1], kc[0], kc[1], kc[2], vc[0], vc[1],
+                         vc[2])
+    launch("vt_rotary_cache", _build.load().vt_rotary_cache, dev.index, q.data_ptr(), q_out.data_ptr(), k.data_ptr(),
            v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), strides, positions.data_ptr(), slots.data_ptr(),
-           freqs.turns.data_ptr(), freqs.factor, int(interleaved), T, Hq, Hkv, D, freqs.rot_dim, k_cache.shape[0],
-           k_cache.shape[1], code)
+           freqs.turns.data_ptr(), freqs.factor, bool(interleaved), T, Hq, Hkv, D, freqs.rot_dim, cshape[0], cshape[1],
+           code)
     return q_out
 
 

@@ -14,7 +14,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _build
-from ._launch import launch, need, same_device, vector
+from ._launch import launch, refuse_devices, vector
 
 MAX_REQUESTS = 4096
 # bits of StepTables.status
@@ -36,10 +36,28 @@ class StepTables(NamedTuple):
 
 def alloc_tables(batch, num_tokens, tree, device):
     """Buffers for step_tables(out=...), e.g. the static ones of a captured step."""
-    ints = torch.empty(2 * batch + 2, dtype=torch.int32, device=device)
-    rows = torch.empty(3 if tree else 2, num_tokens, dtype=torch.int64, device=device)
-    return StepTables(ints[:batch + 1], ints[batch + 1:2 * batch + 1], rows[0], rows[1], rows[2] if tree else None,
-                      ints[2 * batch + 1:])
+    cu, lens, status = torch.empty(2 * batch + 2, dtype=torch.int32, device=device).split((batch + 1, batch, 1))
+    rows = torch.empty((3 if tree else 2, num_tokens), dtype=torch.int64, device=device).unbind(0)
+    return StepTables(cu, lens, rows[0], rows[1], rows[2] if tree else None, status)
+
+
+def _refuse(block_table, held, free_blocks, free_count, cached_lens, new_lens, block_size, T, parents):
+    """Which of step_tables' conditions on its inputs does not hold."""
+    B = held.shape[0] if held.dim() == 1 else -1
+    if not (vector(held, _I32, B) and vector(cached_lens, _I32, B) and vector(new_lens, _I32, B)):
+        raise ValueError("step_tables: held, cached_lens and new_lens must be contiguous int32 [B]")
+    if not (vector(free_blocks, _I32, free_blocks.numel()) and vector(free_count, _I32, 1)):
+        raise ValueError("step_tables: free_blocks must be a contiguous int32 vector and free_count int32 [1]")
+    if T < 0 or block_size < 1:
+        raise ValueError("step_tables: num_tokens >= 0 and block_size >= 1")
+    if B > MAX_REQUESTS:
+        raise ValueError(f"step_tables: at most {MAX_REQUESTS} requests")
+    if parents is not None and not vector(parents, _I32, T):
+        raise ValueError("step_tables: parents must be contiguous int32 [num_tokens]")
+    raise ValueError("step_tables: block_table must be int32 [B, width] with contiguous rows that do not overlap")
+
+
+_I32, _I64 = torch.int32, torch.int64
 
 
 def step_tables(block_table, held, free_blocks, free_count, cached_lens, new_lens, block_size, num_tokens,
@@ -49,30 +67,33 @@ def step_tables(block_table, held, free_blocks, free_count, cached_lens, new_len
     cached_lens [B], new_lens [B] (negative: the request has ended), parents [num_tokens] (index within the request of
     each token's parent, -1 for one that follows the context; None: chains) are read. `out` (alloc_tables) is written
     when given."""
-    B, T = held.shape[0] if held.dim() else -1, int(num_tokens)
-    i32 = torch.int32
-    need(block_table.dim() == 2 and block_table.dtype == i32 and B >= 0 and block_table.shape[0] == B
-         and block_table.shape[1] >= 1 and (B < 2 or block_table.stride(0) >= block_table.shape[1])
-         and block_table.stride(1) == 1, "step_tables: block_table must be int32 [B, width] with contiguous rows")
-    need(vector(held, i32, B) and vector(cached_lens, i32, B) and vector(new_lens, i32, B),
-         "step_tables: held, cached_lens and new_lens must be contiguous int32 [B]")
-    need(vector(free_blocks, i32, free_blocks.numel()) and vector(free_count, i32, 1),
-         "step_tables: free_blocks must be a contiguous int32 vector and free_count int32 [1]")
-    need(T >= 0 and int(block_size) >= 1, "step_tables: num_tokens >= 0 and block_size >= 1")
-    need(B <= MAX_REQUESTS, f"step_tables: at most {MAX_REQUESTS} requests")
-    need(parents is None or vector(parents, i32, T), "step_tables: parents must be contiguous int32 [num_tokens]")
-    if out is None:
-        out = alloc_tables(B, T, parents is not None, held.device)
+    T, bs = int(num_tokens), int(block_size)
+    shape, strides = block_table.shape, block_table.stride()
+    B = shape[0]
+    if not (len(shape) == 2 and shape[1] >= 1 and block_table.dtype == _I32 and strides[1] == 1
+            and (B < 2 or strides[0] >= shape[1]) and vector(held, _I32, B) and vector(cached_lens, _I32, B)
+            and vector(new_lens, _I32, B) and free_blocks.dim() == 1 and vector(free_blocks, _I32, free_blocks.shape[0])
+            and vector(free_count, _I32, 1) and T >= 0 and bs >= 1 and B <= MAX_REQUESTS
+            and (parents is None or vector(parents, _I32, T))):
+        _refuse(block_table, held, free_blocks, free_count, cached_lens, new_lens, bs, T, parents)
+    dev = held.device
+    if out is None:   # alloc_tables as separate tensors, which costs less host time than cutting one up
+        positions = held.new_empty(T, dtype=_I64)
+        out = StepTables(held.new_empty(B + 1), torch.empty_like(held), positions, torch.empty_like(positions),
+                         None if parents is None else torch.empty_like(positions), torch.empty_like(free_count))
     else:
-        i64 = torch.int64
-        need(vector(out.cu, i32, B + 1) and vector(out.seq_lens, i32, B) and vector(out.status, i32, 1)
-             and vector(out.positions, i64, T) and vector(out.slots, i64, T)
-             and (parents is None or (out.mask is not None and vector(out.mask, i64, T))),
-             "step_tables: out does not fit (alloc_tables(B, num_tokens, parents is not None, device))")
+        if not (vector(out.cu, _I32, B + 1) and vector(out.seq_lens, _I32, B) and vector(out.status, _I32, 1)
+                and vector(out.positions, _I64, T) and vector(out.slots, _I64, T)
+                and (parents is None or (out.mask is not None and vector(out.mask, _I64, T)))):
+            raise ValueError("step_tables: out does not fit (alloc_tables(B, num_tokens, parents is not None, device))")
         if parents is None and out.mask is not None:
             out = out._replace(mask=None)
-    dev = same_device("step_tables", held, block_table, cached_lens, new_lens, free_blocks, free_count, parents,
-                      out.cu, out.seq_lens, out.positions, out.slots, out.mask, out.status)
+    if not (dev.type == "cuda" and block_table.device == dev and cached_lens.device == dev and new_lens.device == dev
+            and free_blocks.device == dev and free_count.device == dev and out.cu.device == dev
+            and out.seq_lens.device == dev and out.positions.device == dev and out.slots.device == dev
+            and out.status.device == dev
+            and (parents is None or (parents.device == dev and out.mask.device == dev))):
+        refuse_devices("step_tables", held, block_table, cached_lens, new_lens, free_blocks, free_count, parents, *out)
     if B == 0:
         out.cu.zero_()
         out.positions.zero_()
@@ -81,12 +102,12 @@ def step_tables(block_table, held, free_blocks, free_count, cached_lens, new_len
         if out.mask is not None:
             out.mask.zero_()
         return out
-    launch("vt_step_tables", _build.load().vt_step_tables, dev, block_table.data_ptr(),
-           max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], held.data_ptr(),
-           free_blocks.data_ptr(), free_blocks.shape[0], free_count.data_ptr(), cached_lens.data_ptr(),
-           new_lens.data_ptr(), parents.data_ptr() if parents is not None else None, B, T, int(block_size),
-           out.cu.data_ptr(), out.seq_lens.data_ptr(), out.positions.data_ptr(), out.slots.data_ptr(),
-           out.mask.data_ptr() if out.mask is not None else None, out.status.data_ptr())
+    launch("vt_step_tables", _build.load().vt_step_tables, dev.index, block_table.data_ptr(),
+           max(strides[0], shape[1]), shape[1], held.data_ptr(), free_blocks.data_ptr(), free_blocks.shape[0],
+           free_count.data_ptr(), cached_lens.data_ptr(), new_lens.data_ptr(),
+           None if parents is None else parents.data_ptr(), B, T, bs, out.cu.data_ptr(), out.seq_lens.data_ptr(),
+           out.positions.data_ptr(), out.slots.data_ptr(), None if out.mask is None else out.mask.data_ptr(),
+           out.status.data_ptr())
     return out
 
 
