@@ -185,7 +185,8 @@ int vt_rotary_cache(const void *q, void *q_out, const void *k, const void *v, vo
  * which are the new tokens themselves: token i sees every key before those and, of the new tokens, those with their
  * bit set in mask[cu[b] + i] (int64 [T]), or tokens 0 .. i with mask NULL. Softmax in 32 bits; a token that sees no
  * key gets 0; keys in blocks whose table entry is outside [0, num_blocks) are not seen, whatever the cache holds
- * where nothing is seen. Hq a multiple of Hkv (query head h reads cached head h / (Hq / Hkv)), D a multiple of 8 up to
+ * where nothing is seen. Hq a multiple of Hkv, at most 128 times it (query head h
+ * reads cached head h / (Hq / Hkv)), D a multiple of 8 up to
  * 256, block_size a multiple of 8, caches 16-byte aligned with strides that are multiples of 8 elements, 1 <= max_new
  * <= 64 (tokens of a request past max_new are not computed; rows past cu[B] are left as they were). strides (host, in
  * elements): token and head stride of q and out, then block, row and head stride of k_cache and of v_cache. workspace:

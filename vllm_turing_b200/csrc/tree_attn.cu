@@ -6,7 +6,7 @@
 // it sees, 0 where it sees none. A key in a block whose table entry is out of range is not seen.
 //
 // Rows: the n tokens x G = Hq / Hkv query heads of one cached head share its keys, so they are the rows of one product,
-// 128 to a tile (tcgen05 M = 128; unused rows cost nothing that counts, since rows are independent and the stream of
+// whole tokens of up to 128 rows to a tile (tcgen05 M = 128; unused rows cost nothing that counts, since rows are independent and the stream of
 // keys bounds the kernel below about 250 rows). Per tile of TK keys:
 //   S [128, TK] = Q K^T       tcgen05 kind::f16, both K-major, 128-byte swizzle
 //   P = 2^(S scale log2 e - m) in 16 bits, written over S in tensor memory; m, l: running maximum and sum (32 bits)
@@ -33,8 +33,8 @@
 //
 // CTA: the first warps hold rows; one warp each loads K and V tiles by TMA through the block table (a box holds a power
 // of two of rows that divides block_size, so no box crosses a page), a lane per box, into two rings; one issues the
-// MMAs. The K warp walks the CTA's range and leaves each segment (an item's tiles in the range) in shared memory for
-// the others. The score MMA of tile t + 1 runs while the softmax of tile t does. Every wait is bounded.
+// MMAs; one fetches the next item's Q. The K warp walks the CTA's range and leaves each segment (an item's tiles in the
+// range) in shared memory for the others. The score MMA of tile t + 1 runs while the softmax of tile t does. Every wait is bounded.
 //
 // What nothing sees must not matter, whatever the memory holds: scores are selected, not added to; in the tiles that
 // reach past ctx the rows of V past L are set to zero in shared memory, and infinities and NaN in the step's own rows
@@ -48,6 +48,7 @@ namespace vt {
 constexpr int TA_MAX_NEW = 64;
 constexpr int TA_ROWS = 128;
 constexpr int TA_BARS = 2048;        // barriers and small shared state, bytes
+constexpr int TA_ITEM_COST = 2;      // what an item costs besides its tiles, in tiles, when the ranges are cut
 constexpr float TA_RAISE = 8.0f;     // log2 of the factor by which weights may pass the running maximum
 
 template <int NCH, int REP> struct TaLayout {        // NCH: 64-value chunks of the head
@@ -55,10 +56,15 @@ template <int NCH, int REP> struct TaLayout {        // NCH: 64-value chunks of 
     static constexpr int DP = NCH * 64;
     static constexpr int CH = REP == 1 && NCH <= 2 ? 2 : 1;
     static constexpr bool QT = CH == 1;                            // Q in tensor memory
-    static constexpr int THREADS = 128 * CH + 128;                 // rows, then the K, MMA and V warps and a spare
-    static constexpr int Q_BYTES = QT ? 0 : NCH * TA_ROWS * 128;
-    static constexpr int STAGE_LD = 33;                            // floats a row of the staging area
-    static constexpr int STAGE = REP > 1 ? (TA_ROWS * STAGE_LD * 4 + 1023) / 1024 * 1024 : 0;
+    static constexpr int THREADS = 128 * CH + 128;                 // rows, then the K, MMA, V and Q warps
+    static constexpr int RR = TA_ROWS / REP;                       // rows of an item
+    // QT: the next item's Q waits in shared memory, QC chunks of its rows at a time in QB buffers, for the row warps to
+    // copy; with replicas the buffer also stages their sums when an item ends. Otherwise Q is the MMA's operand there.
+    static constexpr int QC = QT ? (REP < NCH ? REP : NCH) : NCH, QB = QT && REP == 1 ? 2 : 1;
+    static constexpr int Q_ROUND = RR * QC * 128;                  // 16 KB (QT)
+    static constexpr int STAGE_LD = 36;                            // floats a row of the staging area
+    static constexpr int STAGE = REP > 1 ? TA_ROWS * STAGE_LD * 4 : 0;
+    static constexpr int Q_BYTES = (QB * Q_ROUND > STAGE ? QB * Q_ROUND : STAGE + 1023) / 1024 * 1024;
     static constexpr int SLOT = NCH * TK * 128;
     // entries of the rings of segments and of "pages that are not there" words: more than the K ring's slots (half of
     // the 7 that fit, or of 12) + 2, which is how far the K warp can be ahead of the rows
@@ -74,25 +80,27 @@ struct TaArgs {
     const int *table, *cu, *seq_lens;
     const long long *mask;
     long long table_stride;
-    int width, B, T, max_new, Hq, Hkv, G, D, bs, num_blocks;
+    int width, B, T, max_new, Hkv, G, D, bs, num_blocks;
+    int tile_tokens;         // tokens of an item: whole tokens, at most TA_ROWS rows of them
     int box_rows;            // rows a TMA box holds
     int fold, head_step;     // boxes hold all chunks of their rows; chunks from one head to the next (ta_map)
     int cs, gs;              // bytes in a tile from one 64-value chunk to the next, from 8 rows to the next 8
     int k_slots, v_slots;    // slots of the two rings
     int part_rows;           // rows a part in the workspace has room for
-    int q_vec, o_vec;        // 16-byte accesses fit q / out
-    uint32_t q_flip;         // sign bits to flip (a negative scale)
+    int q_map;               // TMA can read q (16-byte aligned)
+    int o_vec;               // 16-byte accesses fit out (2: 32-byte ones)
+    uint32_t negate;         // the MMA takes Q negated (a negative scale)
     float sl2;               // |scale| log2 e
     struct TaDesc *desc;     // [grid]
     float2 *stats;           // [2 grid][part_rows] {m, l}
-    float *parts;            // [2 grid][part_rows][DP]
+    float *parts;            // [2 grid][DP / 4][part_rows][4]
     unsigned *status;
     uint64_t timeout_ns;
 };
 
 // What the joining kernel needs to know of the item that CTA c's range starts inside of.
 struct TaDesc {
-    long long t0, total;     // the item's first unit; units in all
+    long long t0, total;     // the item's first tile, as a unit; units in all
     int split;               // 1: c's range starts inside an item and c is the first to do so
     int nt, ge, cu0, n, h, rt, pad;
 };
@@ -108,8 +116,8 @@ __device__ __forceinline__ TaReq ta_request(const TaArgs &A, int b, int tk) {
     r.n = max(A.cu[b + 1] - r.cu0, 0);
     r.L = max(A.seq_lens[b], 0);
     r.nt = max(1, (int)(((long long)r.L + tk - 1) / tk));
-    r.rtn = (min(r.n, A.max_new) * A.G + TA_ROWS - 1) / TA_ROWS;
-    r.units = (long long)A.Hkv * r.rtn * r.nt;
+    r.rtn = (min(r.n, A.max_new) + A.tile_tokens - 1) / A.tile_tokens;
+    r.units = (long long)A.Hkv * r.rtn * (r.nt + TA_ITEM_COST);
     return r;
 }
 
@@ -121,7 +129,7 @@ struct TaPlan {   // in shared memory
 __device__ __forceinline__ long long ta_range_lo(long long total, int ge, int c) { return total * c / ge; }
 
 struct TaSeg {       // in shared memory
-    long long t0;    // the item's first unit
+    long long t0;    // the item's first tile, as a unit
     int tiles;       // 0: the range has ended
     int b, h, rt, kt0, nt, L, n, cu0;
     int head;        // first segment of the CTA
@@ -129,34 +137,43 @@ struct TaSeg {       // in shared memory
 };
 
 struct TaIter {
-    long long u, hi, base, lo;
+    long long u, hi, base;
     int b;
+    bool begun;
     TaReq r;
     __device__ __forceinline__ TaIter(const TaArgs &A, const TaPlan &p, int tk)
-        : u(p.lo), hi(p.hi), base(p.base0), lo(p.lo), b(p.b0) {
+        : u(p.lo), hi(p.hi), base(p.base0), b(p.b0), begun(false) {
         if (u < hi) r = ta_request(A, b, tk);
     }
+    // An item's units are TA_ITEM_COST without a tile, then its tiles.
     __device__ __forceinline__ void next(const TaArgs &A, int tk, TaSeg &s) {
         s.tiles = 0;
-        if (u >= hi) return;
-        while (u >= base + r.units) {
-            base += r.units;
-            r = ta_request(A, ++b, tk);
+        while (u < hi) {
+            while (u >= base + r.units) {
+                base += r.units;
+                r = ta_request(A, ++b, tk);
+            }
+            const int per = r.nt + TA_ITEM_COST;
+            const long long x = u - base, item = x / per;
+            const int y = (int)(x - item * per), take = (int)min((long long)per - y, hi - u);
+            const int kt0 = max(y - TA_ITEM_COST, 0), kt1 = max(y + take - TA_ITEM_COST, 0);
+            s.t0 = u - y + TA_ITEM_COST;
+            u += take;
+            if (kt1 == kt0) continue;
+            s.b = b;
+            s.kt0 = kt0;
+            s.tiles = kt1 - kt0;
+            s.h = (int)(item / r.rtn);
+            s.rt = (int)(item - (long long)s.h * r.rtn);
+            s.nt = r.nt;
+            s.L = r.L;
+            s.n = r.n;
+            s.cu0 = r.cu0;
+            s.head = !begun;
+            begun = true;
+            s.whole = s.tiles == r.nt;
+            return;
         }
-        const long long x = u - base, item = x / r.nt;
-        s.b = b;
-        s.kt0 = (int)(x - item * r.nt);
-        s.tiles = (int)min((long long)r.nt - s.kt0, hi - u);
-        s.h = (int)(item / r.rtn);
-        s.rt = (int)(item - (long long)s.h * r.rtn);
-        s.nt = r.nt;
-        s.L = r.L;
-        s.n = r.n;
-        s.cu0 = r.cu0;
-        s.t0 = u - s.kt0;
-        s.head = u == lo;
-        s.whole = s.tiles == r.nt;
-        u += s.tiles;
     }
 };
 
@@ -285,7 +302,20 @@ __device__ __forceinline__ void tma_load_5d(void *dst, const CUtensorMap *map, i
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(u), "r"(smem_u32(bar))
         : "memory");
 }
-// N (8, 16 or 32) consecutive tensor-memory columns of the warp's lanes from / to registers.
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+            "r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+// 32 bytes to global memory, 32-byte aligned
+__device__ __forceinline__ void st_global32(void *p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+// N (16 or 32) consecutive tensor-memory columns of the warp's lanes from / to registers.
 template <int N> __device__ __forceinline__ void ta_ld(uint32_t taddr, uint32_t *r) {
     static_assert(N == 16 || N == 32, "columns");
     if constexpr (N == 32) tmem_ld32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r));
@@ -316,26 +346,29 @@ __device__ __forceinline__ uint32_t ta_seen(unsigned long long see, int kk0, int
 template <typename T, int NCH, int REP>
 __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-                     const __grid_constant__ TaArgs A) {
+                     const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ TaArgs A) {
     using Lay = TaLayout<NCH, REP>;
     constexpr int TK = Lay::TK, DP = Lay::DP, CH = Lay::CH;
-    constexpr int ROW_WARPS = 4 * CH, K_WARP = ROW_WARPS, MMA_WARP = ROW_WARPS + 1, V_WARP = ROW_WARPS + 2;
+    constexpr int ROW_WARPS = 4 * CH, K_WARP = ROW_WARPS, MMA_WARP = ROW_WARPS + 1, V_WARP = ROW_WARPS + 2,
+                  Q_WARP = ROW_WARPS + 3;
     constexpr bool QT = Lay::QT;
     constexpr int TA_RING = Lay::RING;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *qs = tc_align1024(smem_raw);
     const int SK = A.k_slots, SV = A.v_slots;
     unsigned char *kring = qs + Lay::Q_BYTES, *vring = kring + (size_t)SK * Lay::SLOT;
-    float *stage = reinterpret_cast<float *>(vring + (size_t)SV * Lay::SLOT);   // [128][STAGE_LD] (REP > 1)
-    uint64_t *kfull = reinterpret_cast<uint64_t *>(vring + (size_t)SV * Lay::SLOT + Lay::STAGE);
+    float *stage = reinterpret_cast<float *>(qs);   // [128][STAGE_LD] (REP > 1)
+    uint64_t *kfull = reinterpret_cast<uint64_t *>(vring + (size_t)SV * Lay::SLOT);
     uint64_t *kempty = kfull + SK;
     uint64_t *vfull = kempty + SK;
     uint64_t *vempty = vfull + SV;
     uint64_t *sfull = vempty + SV;      // [2] scores in S buffer
     uint64_t *pfull = sfull + 2;        // [2] weights over them (and V ready for use), 4 row warps arrive
     uint64_t *pvdone = pfull + 2;       // [2] the MMAs that read them (and added to O) have completed
-    uint64_t *qfull = pvdone + 2;       // [1] Q in place, the row warps arrive
-    uint64_t *drain = qfull + 1;
+    uint64_t *qfull = pvdone + 2;       // [1] Q in place for the MMA (QT: the row warps arrive, else the Q warp)
+    uint64_t *qbfull = qfull + 1;       // [2] QT: Q buffer loaded
+    uint64_t *qbempty = qbfull + 2;     // [2] Q buffer free (QT: the row warps arrive, else the item's last scores)
+    uint64_t *drain = qbempty + 2;
     uint64_t *segfull = drain + 1;      // [TA_RING]
     TaSeg *segs = reinterpret_cast<TaSeg *>(segfull + TA_RING);   // [TA_RING]
     TaPlan *plan = reinterpret_cast<TaPlan *>(segs + TA_RING);
@@ -362,13 +395,16 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             mbar_init(&sfull[b], 1);
             mbar_init(&pfull[b], 4);
             mbar_init(&pvdone[b], 1);
+            mbar_init(&qbfull[b], 1);
+            mbar_init(&qbempty[b], QT ? ROW_WARPS : 1);
         }
-        mbar_init(qfull, ROW_WARPS);
+        mbar_init(qfull, QT ? ROW_WARPS : 1);
         mbar_init(drain, 1);
         for (int i = 0; i < 4; ++i) wild[i] = 0;
         fence_mbar_init();
         tma_prefetch_desc(&tmap_k);
         tma_prefetch_desc(&tmap_v);
+        if (A.q_map) tma_prefetch_desc(&tmap_q);
     }
     if (warp == MMA_WARP) {
         tmem_alloc(tmem_slot, 512);
@@ -460,7 +496,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         // ---------------- MMA issuer ----------------
         // The whole warp runs the loop on warp-uniform values and one elected lane issues: operands stay in uniform
         // registers. (A loop inside `if (lane == 0)` took about 120 cycles an MMA to issue, more than the MMAs.)
-        constexpr uint32_t id_s = idesc_f16<T>(TA_ROWS, TK);
+        const uint32_t id_s = idesc_f16<T>(TA_ROWS, TK) | (A.negate << 13);
         constexpr uint32_t id_o = idesc_f16<T>(TA_ROWS, DP) | (1u << 16);   // B (V) is MN-major
         const uint32_t tb = __shfl_sync(0xffffffffu, tmem_base, 0), kring0 = smem_u32(kring), vring0 = smem_u32(vring);
         const uint64_t qd = sw128_desc(smem_u32(qs));
@@ -497,6 +533,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             ok = wait(qfull, (uint32_t)seg & 1u, 0x230u) && scores(g);
             for (int t = 0; ok && t < N; ++t, ++g) {
                 if (t + 1 < N) ok = scores(g + 1);
+                else if (!QT) umma_commit_e(&qbempty[0]);
                 ok = ok && wait(&pfull[g & 1], (uint32_t)(g >> 1) & 1u, 0x240u);
                 ok = ok && wait(&vfull[vs], vphase, 0x250u);
                 if (!ok) break;
@@ -514,6 +551,46 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         }
         umma_commit_e(drain);   // every MMA issued has completed once it flips
         warp_wait(drain, 0u, globaltimer() + A.timeout_ns);
+    } else if (warp == Q_WARP) {
+        // ---------------- Q of the items ----------------
+        // [chunk][row] of 128 bytes (64 values), swizzled: one TMA box a chunk (its tokens past the request's end give
+        // rows that nothing uses), or, for a q that TMA cannot read, element by element.
+        constexpr int QC = Lay::QC, QB = Lay::QB;
+        int round = 0;
+        bool ok = true;
+        for (int seg = 0; ok; ++seg) {
+            ok = warp_wait(&segfull[seg % TA_RING], (uint32_t)(seg / TA_RING) & 1u, deadline);
+            const TaSeg &sg = segs[seg % TA_RING];
+            if (!ok || sg.tiles == 0) break;
+            const int tok0 = sg.cu0 + sg.rt * A.tile_tokens, h0 = sg.h * A.G;
+            const int rows = min(A.tile_tokens, A.max_new) * A.G;
+            for (int c0 = 0; ok && c0 < NCH; c0 += QC, ++round) {
+                const int b = round % QB, nc = min(QC, NCH - c0);
+                uint64_t *bar = QT ? &qbfull[b] : qfull;
+                ok = warp_wait(&qbempty[b], ((uint32_t)(round / QB) & 1u) ^ 1u, deadline);
+                if (!ok) break;
+                unsigned char *buf = qs + b * Lay::Q_ROUND;
+                if (A.q_map) {
+                    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(nc * rows * 128));
+                    __syncwarp();
+                    if (lane < nc) tma_load_3d(buf + lane * (Lay::RR * 128), &tmap_q, (c0 + lane) * 64, h0, tok0, bar);
+                    continue;
+                }
+                for (int i = lane; i < nc * rows * 64; i += 32) {
+                    const int c = i / (rows * 64), r = i / 64 % rows, d = i % 64, t = r / A.G, tok = tok0 + t;
+                    T x = f2t<T>(0.0f);
+                    if ((c0 + c) * 64 + d < A.D && tok >= 0 && tok < A.T)
+                        x = reinterpret_cast<const T *>(A.q)[(long long)tok * A.q_t + (long long)(h0 + r - t * A.G) * A.q_h +
+                                                             (c0 + c) * 64 + d];
+                    reinterpret_cast<T *>(buf + c * (Lay::RR * 128) + r * 128 + (((d >> 3) ^ (r & 7)) << 4))[d & 7] = x;
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar);
+            }
+        }
+        if (!ok && lane == 0) report(A.status, ST_PIPE_TIMEOUT | 0x2b0u);
+        __syncwarp();
     } else if (warp < ROW_WARPS) {
         // ---------------- rows: softmax and output ----------------
         const int q4 = warp & 3, grp = warp >> 2;
@@ -530,74 +607,40 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             }
             tc_fence_after();
         };
-        int g = 0, seg = 0;
-        // the next segment, if there is one, and its Q
+        int g = 0, seg = 0, qround = 0;
+        // the next segment, if there is one, and its Q into tensor memory
         auto open = [&]() {
             wait(&segfull[seg % TA_RING], (uint32_t)(seg / TA_RING) & 1u, 0x258u);
-            const TaSeg &s = segs[seg % TA_RING];
-            if (threadIdx.x == 0) *more = !dead && s.tiles != 0;   // one thread decides: the warps' barriers must match
-            named_sync(TC_EPI_BAR, 128 * CH);
+            if (threadIdx.x == 0) *more = !dead && segs[seg % TA_RING].tiles != 0;   // one thread decides: the warps'
+            named_sync(TC_EPI_BAR, 128 * CH);                                        // barriers must match
             if (!*more) return false;
-            const int live = min(min(s.n, A.max_new) * A.G - s.rt * TA_ROWS, TA_ROWS);
-            const T *q = reinterpret_cast<const T *>(A.q) + (long long)s.cu0 * A.q_t + (long long)s.h * A.G * A.q_h;
-            // row r's values, or NULL for a row that is none
-            auto row_of = [&](int r) -> const T * {
-                const int gr = s.rt * TA_ROWS + r, i = gr / A.G, tok = s.cu0 + i;
-                return r < live && tok >= 0 && tok < A.T ? q + (long long)i * A.q_t + (long long)(gr - i * A.G) * A.q_h
-                                                         : nullptr;
-            };
-            auto vector = [&](const T *src, int d) {   // 8 values
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (src && d < A.D) {
-                    const uint16_t *e = reinterpret_cast<const uint16_t *>(src + d);
-                    x = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
-                                   e[6] | (uint32_t)e[7] << 16);
-                }
-                return x;
-            };
-            if constexpr (QT) {   // a thread's own row, 64 values (32 columns) at a time
-                if ((REP > 1 ? 0 : q4 * 32) < live) {
-                    const T *src = row_of(row);
+            if constexpr (QT) {
+                constexpr int QC = Lay::QC, QB = Lay::QB;
 #pragma unroll
-                    for (int c = 0; c < NCH; ++c) {
-                        uint4 x[8];
-                        if (A.q_vec) {   // the loads of a chunk in flight together
+                for (int c0 = 0; c0 < NCH; c0 += QC, ++qround) {
+                    const int b = qround % QB;
+                    wait(&qbfull[b], (uint32_t)(qround / QB) & 1u, 0x2b8u);
+                    const unsigned char *buf = qs + b * Lay::Q_ROUND + row * 128;
 #pragma unroll
-                            for (int v = 0; v < 8; ++v)
-                                x[v] = src && c * 64 + v * 8 < A.D
-                                           ? *reinterpret_cast<const uint4 *>(src + c * 64 + v * 8)
-                                           : make_uint4(0, 0, 0, 0);
-                        } else {
-#pragma unroll
-                            for (int v = 0; v < 8; ++v) x[v] = vector(src, c * 64 + v * 8);
-                        }
+                    for (int c = 0; c < QC && c0 + c < NCH; ++c) {   // rows past the item's hold anything
                         uint32_t w[32];
 #pragma unroll
                         for (int v = 0; v < 8; ++v) {
-                            w[4 * v] = x[v].x ^ A.q_flip, w[4 * v + 1] = x[v].y ^ A.q_flip;
-                            w[4 * v + 2] = x[v].z ^ A.q_flip, w[4 * v + 3] = x[v].w ^ A.q_flip;
+                            const uint4 x = *reinterpret_cast<const uint4 *>(buf + c * (Lay::RR * 128) +
+                                                                             ((v ^ (row & 7)) << 4));
+                            w[4 * v] = x.x, w[4 * v + 1] = x.y, w[4 * v + 2] = x.z, w[4 * v + 3] = x.w;
                         }
-                        tmem_st32(lane_base + Lay::Q_COL + 32 * c, w);
+                        tmem_st32(lane_base + Lay::Q_COL + 32 * (c0 + c), w);
                     }
-                    tmem_st_wait();
+                    // with replicas the buffer is the staging area too: free once the item before is written
+                    __syncwarp();
+                    if (lane == 0 && (REP == 1 || seg == 0 || c0 + QC < NCH)) mbar_arrive(&qbempty[b]);
                 }
+                tmem_st_wait();
                 tc_fence_before();
-            } else {   // all threads, swizzled as TMA would lay the rows out
-                constexpr int NV = NCH * 8;
-#pragma unroll 4
-                for (int idx = threadIdx.x; idx < live * NV; idx += 128 * CH) {
-                    const int r = idx / NV, v = idx - r * NV;
-                    const T *src = row_of(r);
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (!A.q_vec) x = vector(src, v * 8);
-                    else if (src && v * 8 < A.D) x = *reinterpret_cast<const uint4 *>(src + v * 8);
-                    *reinterpret_cast<uint4 *>(qs + (v >> 3) * (TA_ROWS * 128) + r * 128 + (((v & 7) ^ (r & 7)) << 4)) =
-                        make_uint4(x.x ^ A.q_flip, x.y ^ A.q_flip, x.z ^ A.q_flip, x.w ^ A.q_flip);
-                }
-                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(qfull);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(qfull);
             return true;
         };
         bool has = open();
@@ -622,8 +665,8 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         while (has) {
             const TaSeg &sg = segs[seg % TA_RING];
             const int N = sg.tiles, L = sg.L, ctx = L - sg.n, kt0 = sg.kt0, g0 = g;
-            const int live = min(min(sg.n, A.max_new) * A.G - sg.rt * TA_ROWS, TA_ROWS);
-            const int gr = sg.rt * TA_ROWS + row, tok_i = gr / A.G, tok = sg.cu0 + tok_i;
+            const int live = min(min(sg.n, A.max_new) - sg.rt * A.tile_tokens, A.tile_tokens) * A.G;
+            const int row_i = row / A.G, tok_i = sg.rt * A.tile_tokens + row_i, tok = sg.cu0 + tok_i;
             const bool mine = row < live && tok >= 0 && tok < A.T;
             const bool warp_live = (REP > 1 ? 0 : q4 * 32) < live;
             unsigned long long see = 0;
@@ -642,33 +685,38 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                 wait(&sfull[buf], use & 1u, 0x260u);
                 const uint32_t gone = bad[g % TA_RING];
                 if (warp_live) {
-                    // W keys at a time; a thread with more (CH = 2, whose ten warps leave it 168 registers) reads its
-                    // scores twice
-                    constexpr int W = CH == 2 ? 32 : CPT, LD = CPT < 32 ? CPT : 32;
-                    float x[W < 32 ? 32 : W];
-                    auto read = [&](int c0) {
+                    // W keys at a time; a thread with more (CH = 2, which leaves it 168 registers) reads its scores
+                    // twice, a chunk ahead of the one it works on
+                    constexpr int W = CH == 2 ? 32 : CPT, LD = CPT < 32 ? CPT : 32, NW = CPT / W;
+                    float x[NW > 1 ? 2 : 1][W < 32 ? 32 : W];
+                    auto fetch = [&](int i, int n) {
 #pragma unroll
                         for (int c = 0; c < W; c += LD)
-                            ta_ld<LD>(s_col + (uint32_t)(part * CPT + c0 + c), reinterpret_cast<uint32_t *>(&x[c]));
-                        tmem_ld_wait();
+                            ta_ld<LD>(s_col + (uint32_t)(part * CPT + n * W + c), reinterpret_cast<uint32_t *>(&x[i][c]));
+                    };
+                    auto hide = [&](int i, int n) {
                         if (past || gone != 0) {
 #pragma unroll
                             for (int c = 0; c < W; c += LD) {
-                                const int kk = part * CPT + c0 + c;
+                                const int kk = part * CPT + n * W + c;
                                 uint32_t vis = ta_seen(see, k0 + kk, ctx);
                                 const uint32_t g4 = (gone >> (kk / 8)) & 15u;
                                 vis &= ~(((g4 * 0x00204081u) & 0x01010101u) * 255u);
 #pragma unroll
-                                for (int j = 0; j < LD; ++j) x[c + j] = (vis >> j) & 1u ? x[c + j] : -INFINITY;
+                                for (int j = 0; j < LD; ++j) x[i][c + j] = (vis >> j) & 1u ? x[i][c + j] : -INFINITY;
                             }
                         }
                     };
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    fetch(0, 0);
 #pragma unroll
-                    for (int c0 = 0; c0 < CPT; c0 += W) {
-                        read(c0);
+                    for (int n = 0; n < NW; ++n) {
+                        const int i = NW > 1 ? n & 1 : 0;
+                        tmem_ld_wait();
+                        if (NW > 1) fetch(i ^ 1, (n + 1) % NW);
+                        hide(i, n);
 #pragma unroll
-                        for (int j = 0; j < W; ++j) mx[j & 3] = fmaxf(mx[j & 3], x[j]);
+                        for (int j = 0; j < W; ++j) mx[j & 3] = fmaxf(mx[j & 3], x[i][j]);
                     }
                     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                     const float tm = top * A.sl2;   // sl2 > 0
@@ -695,18 +743,23 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     uint32_t w[W / 2];
 #pragma unroll
-                    for (int c0 = 0; c0 < CPT; c0 += W) {
-                        if (CPT > W) read(c0);
+                    for (int n = 0; n < NW; ++n) {
+                        const int i = NW > 1 ? n & 1 : 0;
+                        if (NW > 1) {
+                            tmem_ld_wait();
+                            if (n + 1 < NW) fetch(i ^ 1, n + 1);
+                            hide(i, n);
+                        }
 #pragma unroll
                         for (int j = 0; j < W; j += 2) {   // a hidden key: 2^-inf = 0
-                            const float a = ta_exp2(__fmaf_rn(x[j], A.sl2, off));
-                            const float b = ta_exp2(__fmaf_rn(x[j + 1], A.sl2, off));
+                            const float a = ta_exp2(__fmaf_rn(x[i][j], A.sl2, off));
+                            const float b = ta_exp2(__fmaf_rn(x[i][j + 1], A.sl2, off));
                             sum[j & 2] += a;
                             sum[(j & 2) + 1] += b;
                             w[j >> 1] = ta_pack<T>(a, b);
                         }
                         // over scores already read: key k's column of P is k / 2
-                        if constexpr (REP == 1) ta_st<W / 2>(s_col + (uint32_t)(c0 / 2), w);
+                        if constexpr (REP == 1) ta_st<W / 2>(s_col + (uint32_t)(n * W / 2), w);
                     }
                     if constexpr (REP > 1) {
                         // the replica's CPT / 2 columns of P, zeros in the others'
@@ -755,8 +808,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&pfull[buf]);
             }
-            // the next item's Q may go in once this one's last scores are done
-            if (CH == 2) wait(&sfull[(g - 1) & 1], (uint32_t)((g - 1) >> 1) & 1u, 0x298u);
+            // the next item's Q may go in: this one's last scores are done
             ++seg;
             has = open();
             wait(&pvdone[(g - 1) & 1], (uint32_t)((g - 1) >> 1) & 1u, 0x2a0u);
@@ -804,9 +856,9 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             const unsigned long long wn = see & (wv[0] | (unsigned long long)wv[1] << 32);
             const bool whole = sg.whole;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const size_t prow = (size_t)(2 * blockIdx.x + (sg.head ? 0 : 1)) * A.part_rows + row;
+            const size_t slot = (size_t)(2 * blockIdx.x + (sg.head ? 0 : 1));
             T *dst = reinterpret_cast<T *>(A.out) + (long long)tok * A.o_t +
-                     (long long)(sg.h * A.G + gr - tok_i * A.G) * A.o_h;
+                     (long long)(sg.h * A.G + row - row_i * A.G) * A.o_h;
             // NV values of the row from column c: the parts go to the workspace in 32 bits, a whole item's to the output
             auto put = [&](auto &o, int c) {
                 constexpr int NV = sizeof(o) / sizeof(float);
@@ -826,27 +878,34 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                         }
                     }
                 }
-                if (!whole) {
-                    float4 *w = reinterpret_cast<float4 *>(A.parts + prow * DP + c);
+                if (!whole) {   // [slot][column / 4][row][4]: a warp's rows side by side
+                    float4 *w = reinterpret_cast<float4 *>(A.parts) + (slot * (DP / 4) + c / 4) * A.part_rows + row;
 #pragma unroll
                     for (int e = 0; e < NV / 4; ++e)
-                        w[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        w[(size_t)e * A.part_rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                     return;
                 }
+                uint32_t w[NV / 2 < 12 ? 12 : NV / 2];
+#pragma unroll
+                for (int e = 0; e < NV / 2; ++e) w[e] = ta_pack<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
 #pragma unroll
                 for (int e = 0; e < NV; e += 8) {
                     if (c + e >= A.D) break;
-                    uint32_t w[4];
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) w[h] = ta_pack<T>(o[e + 2 * h] * inv, o[e + 2 * h + 1] * inv);
+                    if constexpr (NV >= 16) {   // 32 bytes at a time where they fit
+                        if (A.o_vec == 2 && (e & 8 || c + e + 8 < A.D)) {
+                            if (e & 8) continue;
+                            st_global32(dst + c + e, *reinterpret_cast<const uint32_t(*)[8]>(&w[e / 2]));
+                            continue;
+                        }
+                    }
                     if (A.o_vec) {
-                        *reinterpret_cast<uint4 *>(dst + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<uint4 *>(dst + c + e) = make_uint4(w[e / 2], w[e / 2 + 1], w[e / 2 + 2], w[e / 2 + 3]);
                     } else {
                         uint16_t *d16 = reinterpret_cast<uint16_t *>(dst + c + e);
 #pragma unroll
                         for (int h = 0; h < 4; ++h) {
-                            d16[2 * h] = (uint16_t)w[h];
-                            d16[2 * h + 1] = (uint16_t)(w[h] >> 16);
+                            d16[2 * h] = (uint16_t)w[e / 2 + h];
+                            d16[2 * h + 1] = (uint16_t)(w[e / 2 + h] >> 16);
                         }
                     }
                 }
@@ -854,28 +913,40 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             if constexpr (REP > 1) {
                 // 32 columns at a time through shared memory; a thread then adds up REP replicas of 32 / REP of them
                 constexpr int NV = 32 / REP;
+                float o[32];
+                tmem_ld32(lane_base, *reinterpret_cast<uint32_t(*)[32]>(o));
 #pragma unroll 1
                 for (int c = 0; c < DP; c += 32) {
-                    float o[32];
-                    tmem_ld32(lane_base + (uint32_t)c, *reinterpret_cast<uint32_t(*)[32]>(o));
                     tmem_ld_wait();
+                    float4 *mine4 = reinterpret_cast<float4 *>(stage + tid * Lay::STAGE_LD);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) stage[tid * Lay::STAGE_LD + e] = f0 == 0.0f ? 0.0f : o[e] * f0;
+                    for (int e = 0; e < 8; ++e)
+                        mine4[e] = f0 == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                              : make_float4(o[4 * e] * f0, o[4 * e + 1] * f0, o[4 * e + 2] * f0,
+                                                            o[4 * e + 3] * f0);
+                    if (c + 32 < DP) tmem_ld32(lane_base + (uint32_t)(c + 32), *reinterpret_cast<uint32_t(*)[32]>(o));
                     named_sync(TC_EPI_BAR, 128);
                     if (mine && !dead) {
                         float r[NV];
 #pragma unroll
-                        for (int e = 0; e < NV; ++e) {
-                            r[e] = 0.0f;
+                        for (int e = 0; e < NV; ++e) r[e] = 0.0f;
 #pragma unroll
-                            for (int k = 0; k < REP; ++k)
-                                r[e] += stage[(k * RR + row) * Lay::STAGE_LD + part * NV + e];
+                        for (int k = 0; k < REP; ++k) {
+                            const float4 *p = reinterpret_cast<const float4 *>(stage + (k * RR + row) * Lay::STAGE_LD) +
+                                              part * (NV / 4);
+#pragma unroll
+                            for (int e = 0; e < NV / 4; ++e) {
+                                const float4 y = p[e];
+                                r[4 * e] += y.x, r[4 * e + 1] += y.y, r[4 * e + 2] += y.z, r[4 * e + 3] += y.w;
+                            }
                         }
                         put(r, c + part * NV);
                     }
                     named_sync(TC_EPI_BAR, 128);
                 }
-                if (!whole && mine && part == 0) A.stats[prow] = make_float2(m, l);
+                if (!whole && mine && part == 0) A.stats[slot * A.part_rows + row] = make_float2(m, l);
+                __syncwarp();
+                if (has && lane == 0) mbar_arrive(&qbempty[0]);
             } else if (warp_live) {
                 constexpr int HALF = CH == 2 ? DP / 2 : DP;   // a group's share of the columns
 #pragma unroll 1
@@ -896,7 +967,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                     }
                     if (mine && !dead) put(o, c);
                 }
-                if (!whole && mine && grp == 0) A.stats[prow] = make_float2(m, l);
+                if (!whole && mine && grp == 0) A.stats[slot * A.part_rows + row] = make_float2(m, l);
             }
             tc_fence_before();
             if (CH == 2) named_sync(TC_EPI_BAR, 256);   // both groups have read both O
@@ -912,16 +983,16 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
 }
 
 // Joins the parts of the items that a range boundary cuts. Each block reads which CTAs start inside an item, as the
-// first to do so (desc.split), and lists them; the blocks then share out the (item, row) pairs, a row a group of WPR
-// warps: all 8 warps of the block where there are few rows (one token over a long context is cut into many parts), one
-// warp where there are many. A row's contributors are the CTAs c - 1 .. c1 in order; the warps' sums add up in warp
-// order.
-constexpr int TJ_THREADS = 256, TJ_WARPS = TJ_THREADS / 32;
+// first to do so (desc.split), and lists them; the blocks then share out the (item, 32 rows, 8 columns) tasks, a lane a
+// row. A task is a warp's, or that of 2, 4 or 8 warps of a block, which share its contributors, where there are few
+// tasks (one token over a long context is cut into many parts). A row's contributors are the CTAs c - 1 .. c1 in order;
+// the warps' sums add up in warp order.
+constexpr int TJ_THREADS = 256, TJ_WARPS = TJ_THREADS / 32, TJ_COLS = 8;
 template <typename T, int NCH>
 __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_constant__ TaArgs A, int ctas) {
-    constexpr int DP = NCH * 64, E = DP / 32;
-    __shared__ float acc_sm[TJ_WARPS - 1][DP];
-    __shared__ float l_sm[TJ_WARPS];
+    constexpr int DP = NCH * 64, CBS = DP / TJ_COLS;
+    __shared__ float acc_sm[TJ_WARPS][TJ_COLS][32];
+    __shared__ float2 ml_sm[TJ_WARPS][32];
     __shared__ short list[TJ_THREADS];
     __shared__ int found[TJ_WARPS];
     pdl_launch_dependents();
@@ -940,72 +1011,82 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
         }
         if (cut) list[at] = (short)tid;
         __syncthreads();
-        const int rows = A.part_rows, wpr = items * rows <= 4 * (int)gridDim.x ? TJ_WARPS : 1;
-        const int groups = TJ_WARPS / wpr, wr = wpr > 1 ? warp : 0;
-        for (int w0 = blockIdx.x * groups; w0 < items * rows; w0 += gridDim.x * groups) {
-            const int task = w0 + (wpr > 1 ? 0 : warp), item = task / rows, r = task - item * rows;
-            const bool some = task < items * rows;
-            const int c = base + list[some ? item : 0];
-            const TaDesc d = A.desc[c];
-            const int gr = d.rt * TA_ROWS + r, i = gr / A.G, tok = d.cu0 + i;
-            const bool mine = some && r < min(min(d.n, A.max_new) * A.G - d.rt * TA_ROWS, TA_ROWS) && tok >= 0 && tok < A.T;
-            float acc[E], l = 0.0f;
+        const int rows = A.part_rows, rbs = (rows + 31) / 32, per = rbs * CBS, tasks = items * per;
+        int wpr = TJ_WARPS;
+        while (wpr > 1 && (long long)tasks * wpr > (long long)gridDim.x * TJ_WARPS) wpr >>= 1;
+        const int groups = TJ_WARPS / wpr, grp = warp / wpr, wr = warp - grp * wpr;
+        for (int w0 = blockIdx.x * groups; w0 < tasks; w0 += gridDim.x * groups) {
+            const int task = w0 + grp, item = task / per, q = task - item * per, cb = q % CBS;
+            const int r = q / CBS * 32 + lane;
+            float acc[TJ_COLS], l = 0.0f, m = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-            if (mine) {
-                const int first = d.t0 == ta_range_lo(d.total, d.ge, c - 1) ? 2 * (c - 1) : 2 * (c - 1) + 1;
+            for (int e = 0; e < TJ_COLS; ++e) acc[e] = 0.0f;
+            T *dst = nullptr;
+            if (task < tasks) {
+                const int c = base + list[item];
+                const TaDesc d = A.desc[c];
+                const int i = r / A.G, tok = d.cu0 + d.rt * A.tile_tokens + i;
+                if (i < min(min(d.n, A.max_new) - d.rt * A.tile_tokens, A.tile_tokens) && tok >= 0 && tok < A.T)
+                    dst = reinterpret_cast<T *>(A.out) + (long long)tok * A.o_t +
+                          (long long)(d.h * A.G + r - i * A.G) * A.o_h + cb * TJ_COLS;
+                const int first = ta_range_lo(d.total, d.ge, c - 1) >= d.t0 - TA_ITEM_COST ? 2 * (c - 1) : 2 * (c - 1) + 1;
                 const long long last = d.t0 + d.nt - 1;
-                int c1 = (int)(last * d.ge / d.total);   // the CTA holding the item's last unit
+                int c1 = (int)(last * d.ge / d.total);   // the CTA holding the item's last tile
                 while (c1 + 1 < d.ge && ta_range_lo(d.total, d.ge, c1 + 1) <= last) ++c1;
                 const int nc = c1 - (c - 1) + 1;
-                auto slot = [&](int j) { return (size_t)(j == 0 ? first : 2 * (c - 1 + j)) * rows + r; };
-                float M = -INFINITY;
-                for (int j = lane; j < nc; j += 32) M = fmaxf(M, A.stats[slot(j)].x);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-                if (M == -INFINITY) M = 0.0f;
+                if (dst) {
 #pragma unroll 4
-                for (int j = wr; j < nc; j += wpr) {
-                    const size_t s = slot(j);
-                    const float2 st = A.stats[s];
-                    float2 v[E / 2];
-                    const float2 *p = reinterpret_cast<const float2 *>(A.parts + s * DP);
+                    for (int j = wr; j < nc; j += wpr) {
+                        const size_t s = j == 0 ? first : 2 * (c - 1 + j);
+                        const float2 st = A.stats[s * rows + r];
+                        const float4 *p = reinterpret_cast<const float4 *>(A.parts) + (s * (DP / 4) + cb * 2) * rows + r;
+                        const float4 a = p[0], b = p[rows];
+                        const float v[TJ_COLS] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                        const float mn = fmaxf(m, st.x), mz = mn == -INFINITY ? 0.0f : mn;
+                        const float f = ta_exp2(m - mz), w = ta_exp2(st.x - mz);
+                        m = mn;
+                        l = l * f + w * st.y;
 #pragma unroll
-                    for (int e = 0; e < E / 2; ++e) v[e] = p[lane + 32 * e];
-                    const float w = ta_exp2(st.x - M);
-                    l += w * st.y;
-#pragma unroll
-                    for (int e = 0; e < E / 2; ++e) {   // a part without keys may hold anything
-                        acc[2 * e] = w != 0.0f ? __fmaf_rn(w, v[e].x, acc[2 * e]) : acc[2 * e];
-                        acc[2 * e + 1] = w != 0.0f ? __fmaf_rn(w, v[e].y, acc[2 * e + 1]) : acc[2 * e + 1];
+                        for (int e = 0; e < TJ_COLS; ++e) {   // a part without keys may hold anything
+                            const float o = f != 0.0f ? acc[e] * f : 0.0f;
+                            acc[e] = w != 0.0f ? __fmaf_rn(w, v[e], o) : o;
+                        }
                     }
                 }
             }
             if (wpr > 1) {
-                if (wr > 0) {
+                ml_sm[warp][lane] = make_float2(m, l);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) acc_sm[wr - 1][32 * e + lane] = acc[e];
-                }
-                if (lane == 0) l_sm[wr] = l;
+                for (int e = 0; e < TJ_COLS; ++e) acc_sm[warp][e][lane] = acc[e];
                 __syncthreads();
                 if (wr == 0) {
-                    for (int w = 1; w < wpr; ++w) {
-                        l += l_sm[w];
+                    for (int w = warp + 1; w < warp + wpr; ++w) {
+                        const float2 st = ml_sm[w][lane];
+                        const float mn = fmaxf(m, st.x), mz = mn == -INFINITY ? 0.0f : mn;
+                        const float f = ta_exp2(m - mz), g = ta_exp2(st.x - mz);
+                        m = mn;
+                        l = l * f + g * st.y;
 #pragma unroll
-                        for (int e = 0; e < E; ++e) acc[e] += acc_sm[w - 1][32 * e + lane];
+                        for (int e = 0; e < TJ_COLS; ++e) acc[e] = acc[e] * f + g * acc_sm[w][e][lane];
                     }
                 }
                 __syncthreads();
             }
-            if (!mine || wr > 0) continue;
+            if (!dst || wr > 0) continue;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            T *dst = reinterpret_cast<T *>(A.out) + (long long)tok * A.o_t + (long long)(d.h * A.G + gr - i * A.G) * A.o_h;
+            uint32_t w[TJ_COLS / 2];
 #pragma unroll
-            for (int e = 0; e < E / 2; ++e) {
-                const int col = 2 * (lane + 32 * e);
-                if (col >= A.D) continue;
-                dst[col] = f2t<T>(acc[2 * e] * inv);
-                dst[col + 1] = f2t<T>(acc[2 * e + 1] * inv);
+            for (int e = 0; e < TJ_COLS / 2; ++e) w[e] = ta_pack<T>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+            if (cb * TJ_COLS >= A.D) continue;
+            if (A.o_vec) {
+                *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+                uint16_t *d16 = reinterpret_cast<uint16_t *>(dst);
+#pragma unroll
+                for (int e = 0; e < TJ_COLS / 2; ++e) {
+                    d16[2 * e] = (uint16_t)w[e];
+                    d16[2 * e + 1] = (uint16_t)(w[e] >> 16);
+                }
             }
         }
         __syncthreads();
@@ -1040,16 +1121,29 @@ static bool ta_map(CUtensorMap *m, const void *base, int D, int bs, int Hkv, int
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static int ta_part_rows(int max_new, int G) { return max_new * G < TA_ROWS ? max_new * G : TA_ROWS; }
+// q [T][Hq][D]; a box is 64 values of the G heads of one cached head, for an item's tokens.
+static bool ta_q_map(CUtensorMap *m, const void *base, int D, int Hq, int T, long long sh, long long st, int G, int tokens) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)Hq, (cuuint64_t)T};
+    cuuint64_t strides[2] = {(cuuint64_t)sh * 2, (cuuint64_t)st * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)tokens}, estr[3] = {1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static int ta_tile_tokens(int G) { return TA_ROWS / G; }
+static int ta_part_rows(int max_new, int G) { return (max_new < ta_tile_tokens(G) ? max_new : ta_tile_tokens(G)) * G; }
 static size_t ta_desc_bytes(int grid) { return ((size_t)grid * sizeof(TaDesc) + 255) & ~(size_t)255; }
 static size_t ta_stats_bytes(int grid, int rows) { return ((size_t)2 * grid * rows * sizeof(float2) + 255) & ~(size_t)255; }
 
 template <typename T, int NCH, int REP>
-static int launch_ta(const CUtensorMap &mk, const CUtensorMap &mv, TaArgs A, cudaStream_t s) {
+static int launch_ta(const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mq, TaArgs A, cudaStream_t s) {
     using Lay = TaLayout<NCH, REP>;
     const int dev = cur_device();
     if (dev < 0 || dev >= VT_MAX_DEV) return VT_EARG;
-    const int fixed = 1024 + TA_BARS + Lay::Q_BYTES + Lay::STAGE;
+    const int fixed = 1024 + TA_BARS + Lay::Q_BYTES;
     int slots = (max_smem_optin(dev) - fixed) / Lay::SLOT;
     if (slots > 12) slots = 12;
     if (slots < 4) return VT_EARG;
@@ -1066,25 +1160,25 @@ static int launch_ta(const CUtensorMap &mk, const CUtensorMap &mv, TaArgs A, cud
         attr[dev] = true;
     }
     const int grid = num_sms(dev);
-    if (int rc = launch_k(tree_attn_kernel<T, NCH, REP>, dim3(grid), dim3(Lay::THREADS), smem, s, true, mk, mv, A))
+    if (int rc = launch_k(tree_attn_kernel<T, NCH, REP>, dim3(grid), dim3(Lay::THREADS), smem, s, true, mk, mv, mq, A))
         return rc;
     if (grid < 2) return 0;
-    return launch_k(tree_join_kernel<T, NCH>, dim3(2 * grid), dim3(TJ_THREADS), 0, s, true, A, grid);
+    return launch_k(tree_join_kernel<T, NCH>, dim3(4 * grid), dim3(TJ_THREADS), 0, s, true, A, grid);
 }
 
 template <typename T, int NCH>
-static int dispatch_rep(const CUtensorMap &mk, const CUtensorMap &mv, const TaArgs &A, cudaStream_t s) {
+static int dispatch_rep(const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mq, const TaArgs &A, cudaStream_t s) {
     const int rows = A.max_new * A.G;
-    if (rows <= 32) return launch_ta<T, NCH, 4>(mk, mv, A, s);
-    if (rows <= 64) return launch_ta<T, NCH, 2>(mk, mv, A, s);
-    return launch_ta<T, NCH, 1>(mk, mv, A, s);
+    if (rows <= 32) return launch_ta<T, NCH, 4>(mk, mv, mq, A, s);
+    if (rows <= 64) return launch_ta<T, NCH, 2>(mk, mv, mq, A, s);
+    return launch_ta<T, NCH, 1>(mk, mv, mq, A, s);
 }
 
-template <typename T> static int dispatch_ta(const CUtensorMap &mk, const CUtensorMap &mv, const TaArgs &A, cudaStream_t s) {
-    if (A.D <= 64) return dispatch_rep<T, 1>(mk, mv, A, s);
-    if (A.D <= 128) return dispatch_rep<T, 2>(mk, mv, A, s);
-    if (A.D <= 192) return dispatch_rep<T, 3>(mk, mv, A, s);
-    return dispatch_rep<T, 4>(mk, mv, A, s);
+template <typename T> static int dispatch_ta(const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mq, const TaArgs &A, cudaStream_t s) {
+    if (A.D <= 64) return dispatch_rep<T, 1>(mk, mv, mq, A, s);
+    if (A.D <= 128) return dispatch_rep<T, 2>(mk, mv, mq, A, s);
+    if (A.D <= 192) return dispatch_rep<T, 3>(mk, mv, mq, A, s);
+    return dispatch_rep<T, 4>(mk, mv, mq, A, s);
 }
 
 }  // namespace vt
@@ -1094,7 +1188,7 @@ using namespace vt;
 extern "C" {
 
 size_t vt_tree_attention_ws_bytes(int max_new, int Hq, int Hkv, int D) {
-    if (max_new < 1 || max_new > TA_MAX_NEW || Hkv < 1 || Hq < Hkv || D < 1 || D > 256) return 0;
+    if (max_new < 1 || max_new > TA_MAX_NEW || Hkv < 1 || Hq < Hkv || Hq / Hkv > TA_ROWS || D < 1 || D > 256) return 0;
     const int grid = num_sms(cur_device()), rows = ta_part_rows(max_new, Hq / Hkv), dp = (D + 63) / 64 * 64;
     return ta_desc_bytes(grid) + ta_stats_bytes(grid, rows) + (size_t)2 * grid * rows * dp * sizeof(float);
 }
@@ -1105,7 +1199,7 @@ int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, v
                       long long num_blocks, int block_size, float scale, int dtype, void *workspace, size_t ws_bytes,
                       void *stream) {
     if (!q || !k_cache || !v_cache || !out || !strides || !block_table || !cu || !seq_lens || B < 1 || T < 0 ||
-        max_new < 1 || max_new > TA_MAX_NEW || Hkv < 1 || Hq < Hkv || Hq % Hkv || Hq > (1 << 20) || D < 8 || D > 256 ||
+        max_new < 1 || max_new > TA_MAX_NEW || Hkv < 1 || Hq < Hkv || Hq % Hkv || Hq / Hkv > TA_ROWS || D < 8 || D > 256 ||
         D % 8 || block_size < 8 || block_size % 8 || table_width < 0 || num_blocks < 1 || num_blocks > 0x7ffffffe ||
         (dtype != 0 && dtype != 1) || !workspace || ((uintptr_t)workspace & 255) ||
         ws_bytes < vt_tree_attention_ws_bytes(max_new, Hq, Hkv, D) || ((uintptr_t)k_cache & 15) ||
@@ -1121,7 +1215,7 @@ int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, v
     int box = 8;   // the largest power of two of rows that divides the block, at most a tile
     const int tk = D <= 128 ? 128 : 64;
     while (box * 2 <= tk && block_size % (box * 2) == 0) box *= 2;
-    CUtensorMap mk, mv;
+    CUtensorMap mk, mv, mq;
     const bool fold = D % 64 == 0 && strides[6] % 64 == 0 && strides[9] == strides[6];
     if (!ta_map(&mk, k_cache, D, block_size, Hkv, (int)num_blocks, strides[5], strides[6], strides[4], box, fold) ||
         !ta_map(&mv, v_cache, D, block_size, Hkv, (int)num_blocks, strides[8], strides[9], strides[7], box, fold))
@@ -1147,16 +1241,18 @@ int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, v
     A.B = B;
     A.T = T;
     A.max_new = max_new;
-    A.Hq = Hq;
     A.Hkv = Hkv;
     A.G = Hq / Hkv;
+    A.tile_tokens = ta_tile_tokens(A.G);
     A.D = D;
     A.bs = block_size;
     A.num_blocks = (int)num_blocks;
     A.box_rows = box;
-    A.q_vec = ((uintptr_t)q & 15) == 0 && ((A.q_t | A.q_h) & 7) == 0;
+    A.q_map = ((uintptr_t)q & 15) == 0 && ((A.q_t | A.q_h) & 7) == 0 && A.q_t >= 0 && A.q_h >= 0 &&
+              ta_q_map(&mq, q, D, Hq, T, A.q_h, A.q_t, A.G, max_new < A.tile_tokens ? max_new : A.tile_tokens);
     A.o_vec = ((uintptr_t)out & 15) == 0 && ((A.o_t | A.o_h) & 7) == 0;
-    A.q_flip = scale < 0.0f ? 0x80008000u : 0u;
+    if (A.o_vec && ((uintptr_t)out & 31) == 0 && ((A.o_t | A.o_h) & 15) == 0) A.o_vec = 2;
+    A.negate = scale < 0.0f;
     A.sl2 = fmaxf(fabsf(scale) * 1.4426950408889634f, 1.2e-38f);   // above 0: a hidden key's -inf stays -inf
     A.part_rows = ta_part_rows(max_new, A.G);
     A.timeout_ns = pipe_timeout_ns();
@@ -1165,8 +1261,8 @@ int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, v
     A.desc = (TaDesc *)ws;
     A.stats = (float2 *)(ws + ta_desc_bytes(grid));
     A.parts = (float *)(ws + ta_desc_bytes(grid) + ta_stats_bytes(grid, A.part_rows));
-    if (dtype == 0) return dispatch_ta<__half>(mk, mv, A, s);
-    return dispatch_ta<__nv_bfloat16>(mk, mv, A, s);
+    if (dtype == 0) return dispatch_ta<__half>(mk, mv, mq, A, s);
+    return dispatch_ta<__nv_bfloat16>(mk, mv, mq, A, s);
 }
 
 }  // extern "C"

@@ -8,6 +8,7 @@ from . import _build
 from ._launch import launch, need, refuse_devices, refuse_dtypes, vector
 
 MAX_NEW = 64
+MAX_GROUP = 128   # query heads to a cached head
 
 
 _STRIDES = ctypes.c_longlong * 10
@@ -38,7 +39,8 @@ def _refuse(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask):
          f"tree_attention: the caches must be [num_blocks, block_size, Hkv, {D}] alike")
     nb, bs, Hkv, _ = k_cache.shape
     need(nb >= 1 and bs >= 8 and bs % 8 == 0, "tree_attention: at least one block, block_size a multiple of 8")
-    need(Hkv >= 1 and Hq >= 1 and Hq % Hkv == 0, f"tree_attention: {Hq} query heads over {Hkv} cached heads")
+    need(Hkv >= 1 and Hq >= 1 and Hq % Hkv == 0 and Hq // Hkv <= MAX_GROUP,
+         f"tree_attention: {Hq} query heads over {Hkv} cached heads (a multiple, at most {MAX_GROUP} to one)")
     need(_aligned(k_cache, k_cache.stride()) and _aligned(v_cache, v_cache.stride()),
          "tree_attention: caches 16-byte aligned, last dimension contiguous, other strides multiples of 8")
     need(1 <= max_new <= MAX_NEW, f"tree_attention: max_new must be 1 .. {MAX_NEW}, got {max_new}")
@@ -56,7 +58,7 @@ def tree_attention(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask
     A token sees all keys before the step's own and, of those, the ones whose bit is set in its mask word (int64 [T]);
     without a mask, itself and the ones before it. A token that sees nothing gets 0. max_new (1 .. 64): the largest
     number of tokens of a request in this call. Rows of `out` past the last token are left as they were.
-    D % 8 == 0 up to 256, block_size % 8 == 0, Hq a multiple of Hkv; scale defaults to D ** -0.5."""
+    D % 8 == 0 up to 256, block_size % 8 == 0, Hq a multiple of Hkv (at most 128 times it); scale defaults to D ** -0.5."""
     qshape, cshape, tshape = q.shape, k_cache.shape, block_table.shape
     max_new = int(max_new)
     if not (len(qshape) == 3 and len(cshape) == 4 and len(tshape) == 2):
@@ -66,7 +68,7 @@ def tree_attention(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask
     B = tshape[0]
     qs, ks, vs, ts = q.stride(), k_cache.stride(), v_cache.stride(), block_table.stride()
     if not (qs[2] == 1 and 8 <= D <= 256 and D & 7 == 0 and v_cache.shape == cshape and cshape[3] == D and nb >= 1
-            and bs >= 8 and bs & 7 == 0 and 1 <= Hkv <= Hq and Hq % Hkv == 0 and _aligned(k_cache, ks)
+            and bs >= 8 and bs & 7 == 0 and 1 <= Hkv <= Hq <= MAX_GROUP * Hkv and Hq % Hkv == 0 and _aligned(k_cache, ks)
             and _aligned(v_cache, vs) and 1 <= max_new <= MAX_NEW and vector(seq_lens, torch.int32, B)
             and vector(cu, torch.int32, B + 1) and block_table.dtype == torch.int32
             and (ts[1] == 1 or tshape[1] <= 1) and (mask is None or vector(mask, torch.int64, T))) and T > 0:
