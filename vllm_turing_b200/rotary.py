@@ -97,7 +97,7 @@ def rotary(q, k, positions, freqs, interleaved=False, transpose=False, q_out=Non
     qshape = q.shape
     T, Hq, D = qshape
     if q_out is None:
-        q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+        q_out = torch.empty_like(q)
     if not (_plain(q, qshape) and _plain(q_out, qshape)):
         _heads("rotary: q", q, qshape)
         _heads("rotary: q_out", q_out, qshape)
@@ -107,7 +107,7 @@ def rotary(q, k, positions, freqs, interleaved=False, transpose=False, q_out=Non
         kshape = (T, Hkv, D)
         need(Hkv >= 0, "rotary: k must be [T, heads, D]")
         if k_out is None:
-            k_out = torch.empty(T, Hkv, D, dtype=k.dtype, device=k.device)
+            k_out = torch.empty_like(k)
         if not (_plain(k, kshape) and _plain(k_out, kshape)):
             _heads("rotary: k", k, kshape)
             _heads("rotary: k_out", k_out, kshape)
@@ -148,7 +148,7 @@ def rotary_cache(q, k, v, positions, slots, k_cache, v_cache, freqs, interleaved
     Hkv = k.shape[1]
     kshape = (T, Hkv, D)
     if q_out is None:
-        q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+        q_out = torch.empty_like(q)
     if not (_plain(q, qshape) and _plain(q_out, qshape) and _plain(k, kshape) and _plain(v, kshape) and Hkv >= 1):
         _heads("rotary_cache: q", q, qshape)
         _heads("rotary_cache: q_out", q_out, qshape)

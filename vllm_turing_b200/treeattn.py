@@ -75,7 +75,7 @@ def tree_attention(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask
         _refuse(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask)
     dt, dev = q.dtype, q.device
     if out is None:
-        out = torch.empty(T, Hq, D, dtype=dt, device=dev)
+        out = torch.empty_like(q)
     elif not (out.shape == qshape and (out.stride()[2] == 1 or T == 0)):
         raise ValueError("tree_attention: out must have q's shape and a contiguous last dimension")
     code = _CODE.get(dt)
