@@ -86,23 +86,23 @@ struct TaArgs {
     int fold, head_step;     // boxes hold all chunks of their rows; chunks from one head to the next (ta_map)
     int cs, gs;              // bytes in a tile from one 64-value chunk to the next, from 8 rows to the next 8
     int k_slots, v_slots;    // slots of the two rings
-    int part_rows;           // rows a part in the workspace has room for
+    int rows;                // rows of an item at most
     int q_map;               // TMA can read q (16-byte aligned)
     int o_vec;               // 16-byte accesses fit out (2: 32-byte ones)
     uint32_t negate;         // the MMA takes Q negated (a negative scale)
     float sl2;               // |scale| log2 e
     struct TaDesc *desc;     // [grid]
-    float2 *stats;           // [2 grid][part_rows] {m, l}
-    float *parts;            // [2 grid][DP / 4][part_rows][4]
+    float2 *stats;           // [2 grid][TA_ROWS] {m, l}
+    float *parts;            // [2 grid][DP / 4][TA_ROWS][4]
     unsigned *status;
     uint64_t timeout_ns;
 };
 
 // What the joining kernel needs to know of the item that CTA c's range starts inside of.
 struct TaDesc {
-    long long t0, total;     // the item's first tile, as a unit; units in all
     int split;               // 1: c's range starts inside an item and c is the first to do so
-    int nt, ge, cu0, n, h, rt, pad;
+    int first, parts;        // slot of the item's first part; CTAs that hold parts (then c, c + 1, ..: slots 2 c, 2 c + 2, ..)
+    int tokens, tok0, h;     // the item's tokens, the first one's row, cached head
 };
 
 // ---- the units and a CTA's range of them ---------------------------------------------------------------------------
@@ -126,7 +126,15 @@ struct TaPlan {   // in shared memory
     int b0, ge;
 };
 
-__device__ __forceinline__ long long ta_range_lo(long long total, int ge, int c) { return total * c / ge; }
+// x / y for x, y >= 0: a 64-bit division takes a few hundred cycles, and these stand in the way of the first load
+__device__ __forceinline__ long long ta_div(long long x, int y) {
+    return x >> 31 ? x / y : (long long)((unsigned)x / (unsigned)y);
+}
+// floor(total c / ge)
+__device__ __forceinline__ long long ta_range_lo(long long total, int ge, int c) {
+    const long long q = ta_div(total, ge);
+    return q * c + (unsigned)((int)(total - q * ge) * c) / (unsigned)ge;
+}
 
 struct TaSeg {       // in shared memory
     long long t0;    // the item's first tile, as a unit
@@ -154,7 +162,7 @@ struct TaIter {
                 r = ta_request(A, ++b, tk);
             }
             const int per = r.nt + TA_ITEM_COST;
-            const long long x = u - base, item = x / per;
+            const long long x = u - base, item = ta_div(x, per);
             const int y = (int)(x - item * per), take = (int)min((long long)per - y, hi - u);
             const int kt0 = max(y - TA_ITEM_COST, 0), kt1 = max(y + take - TA_ITEM_COST, 0);
             s.t0 = u - y + TA_ITEM_COST;
@@ -163,7 +171,7 @@ struct TaIter {
             s.b = b;
             s.kt0 = kt0;
             s.tiles = kt1 - kt0;
-            s.h = (int)(item / r.rtn);
+            s.h = (int)ta_div(item, r.rtn);
             s.rt = (int)(item - (long long)s.h * r.rtn);
             s.nt = r.nt;
             s.L = r.L;
@@ -648,18 +656,18 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             A.desc[blockIdx.x].split = 0;
             if (has && segs[0].kt0 > 0) {
                 const TaSeg &x = segs[0];
+                const int c = blockIdx.x, ge = plan->ge;
+                const long long total = plan->total, before = ta_range_lo(total, ge, c - 1), last = x.t0 + x.nt - 1;
+                int c1 = (int)(last * ge / total);   // the CTA holding the item's last tile
+                while (c1 + 1 < ge && ta_range_lo(total, ge, c1 + 1) <= last) ++c1;
                 TaDesc d;
-                d.t0 = x.t0;
-                d.total = plan->total;
-                d.split = x.t0 >= ta_range_lo(plan->total, plan->ge, blockIdx.x - 1);
-                d.nt = x.nt;
-                d.ge = plan->ge;
-                d.cu0 = x.cu0;
-                d.n = x.n;
+                d.split = x.t0 >= before;
+                d.first = 2 * (c - 1) + (before >= x.t0 - TA_ITEM_COST ? 0 : 1);   // its first or last segment
+                d.parts = c1 - c + 2;
+                d.tokens = min(min(x.n, A.max_new) - x.rt * A.tile_tokens, A.tile_tokens);
+                d.tok0 = x.cu0 + x.rt * A.tile_tokens;
                 d.h = x.h;
-                d.rt = x.rt;
-                d.pad = 0;
-                A.desc[blockIdx.x] = d;
+                A.desc[c] = d;
             }
         }
         while (has) {
@@ -878,11 +886,11 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                         }
                     }
                 }
-                if (!whole) {   // [slot][column / 4][row][4]: a warp's rows side by side
-                    float4 *w = reinterpret_cast<float4 *>(A.parts) + (slot * (DP / 4) + c / 4) * A.part_rows + row;
+                if (!whole) {   // a warp's rows side by side
+                    float4 *w = reinterpret_cast<float4 *>(A.parts) + (slot * (DP / 4) + c / 4) * TA_ROWS + row;
 #pragma unroll
                     for (int e = 0; e < NV / 4; ++e)
-                        w[(size_t)e * A.part_rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        w[e * TA_ROWS] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                     return;
                 }
                 uint32_t w[NV / 2 < 12 ? 12 : NV / 2];
@@ -911,42 +919,48 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                 }
             };
             if constexpr (REP > 1) {
-                // 32 columns at a time through shared memory; a thread then adds up REP replicas of 32 / REP of them
-                constexpr int NV = 32 / REP;
-                float o[32];
-                tmem_ld32(lane_base, *reinterpret_cast<uint32_t(*)[32]>(o));
+                // The replicas' sums through shared memory, `width` columns at a time; a thread then adds up the REP
+                // replicas of width / REP of its row's. 32 columns fit the staging area; when the CTA has no further item,
+                // the K and V rings are idle and hold them all. (One loop for both: this runs once per item, from a cold
+                // instruction cache.)
+                const int width = has ? 32 : DP, ld = width + 4;
+                float *area = has ? stage : reinterpret_cast<float *>(kring);
 #pragma unroll 1
-                for (int c = 0; c < DP; c += 32) {
-                    tmem_ld_wait();
-                    float4 *mine4 = reinterpret_cast<float4 *>(stage + tid * Lay::STAGE_LD);
+                for (int c0 = 0; c0 < DP; c0 += width) {
+#pragma unroll 1
+                    for (int c = 0; c < width; c += 64) {
+                        float o[64];
+                        const bool two = c + 32 < width;
+                        tmem_ld32(lane_base + (uint32_t)(c0 + c), *reinterpret_cast<uint32_t(*)[32]>(o));
+                        if (two) tmem_ld32(lane_base + (uint32_t)(c0 + c + 32), *reinterpret_cast<uint32_t(*)[32]>(o + 32));
+                        tmem_ld_wait();
+                        float4 *y = reinterpret_cast<float4 *>(area + tid * ld + c);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        mine4[e] = f0 == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                        for (int e = 0; e < 16; ++e) {
+                            if ((e == 8 && !two) || row >= live) break;   // only the item's rows
+                            y[e] = f0 == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
                                               : make_float4(o[4 * e] * f0, o[4 * e + 1] * f0, o[4 * e + 2] * f0,
                                                             o[4 * e + 3] * f0);
-                    if (c + 32 < DP) tmem_ld32(lane_base + (uint32_t)(c + 32), *reinterpret_cast<uint32_t(*)[32]>(o));
-                    named_sync(TC_EPI_BAR, 128);
-                    if (mine && !dead) {
-                        float r[NV];
-#pragma unroll
-                        for (int e = 0; e < NV; ++e) r[e] = 0.0f;
-#pragma unroll
-                        for (int k = 0; k < REP; ++k) {
-                            const float4 *p = reinterpret_cast<const float4 *>(stage + (k * RR + row) * Lay::STAGE_LD) +
-                                              part * (NV / 4);
-#pragma unroll
-                            for (int e = 0; e < NV / 4; ++e) {
-                                const float4 y = p[e];
-                                r[4 * e] += y.x, r[4 * e + 1] += y.y, r[4 * e + 2] += y.z, r[4 * e + 3] += y.w;
-                            }
                         }
-                        put(r, c + part * NV);
                     }
                     named_sync(TC_EPI_BAR, 128);
+                    if (mine && !dead) {
+#pragma unroll 2
+                        for (int c = part * (width / REP); c < (part + 1) * (width / REP); c += 8) {
+                            float r[8] = {};
+#pragma unroll
+                            for (int k = 0; k < REP; ++k) {
+                                const float4 *y = reinterpret_cast<const float4 *>(area + (k * RR + row) * ld + c);
+                                const float4 a = y[0], b = y[1];
+                                r[0] += a.x, r[1] += a.y, r[2] += a.z, r[3] += a.w;
+                                r[4] += b.x, r[5] += b.y, r[6] += b.z, r[7] += b.w;
+                            }
+                            put(r, c0 + c);
+                        }
+                    }
+                    if (has) named_sync(TC_EPI_BAR, 128);
                 }
-                if (!whole && mine && part == 0) A.stats[slot * A.part_rows + row] = make_float2(m, l);
-                __syncwarp();
-                if (has && lane == 0) mbar_arrive(&qbempty[0]);
+              if (!whole && mine && part == 0) A.stats[slot * TA_ROWS + row] = make_float2(m, l);
             } else if (warp_live) {
                 constexpr int HALF = CH == 2 ? DP / 2 : DP;   // a group's share of the columns
 #pragma unroll 1
@@ -967,7 +981,11 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                     }
                     if (mine && !dead) put(o, c);
                 }
-                if (!whole && mine && grp == 0) A.stats[slot * A.part_rows + row] = make_float2(m, l);
+                if (!whole && mine && grp == 0) A.stats[slot * TA_ROWS + row] = make_float2(m, l);
+            }
+            if constexpr (REP > 1) {   // the staging area is the Q buffer again
+                __syncwarp();
+                if (has && lane == 0) mbar_arrive(&qbempty[0]);
             }
             tc_fence_before();
             if (CH == 2) named_sync(TC_EPI_BAR, 256);   // both groups have read both O
@@ -1011,7 +1029,7 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
         }
         if (cut) list[at] = (short)tid;
         __syncthreads();
-        const int rows = A.part_rows, rbs = (rows + 31) / 32, per = rbs * CBS, tasks = items * per;
+        const int rbs = (A.rows + 31) / 32, per = rbs * CBS, tasks = items * per;
         int wpr = TJ_WARPS;
         while (wpr > 1 && (long long)tasks * wpr > (long long)gridDim.x * TJ_WARPS) wpr >>= 1;
         const int groups = TJ_WARPS / wpr, grp = warp / wpr, wr = warp - grp * wpr;
@@ -1025,22 +1043,17 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
             if (task < tasks) {
                 const int c = base + list[item];
                 const TaDesc d = A.desc[c];
-                const int i = r / A.G, tok = d.cu0 + d.rt * A.tile_tokens + i;
-                if (i < min(min(d.n, A.max_new) - d.rt * A.tile_tokens, A.tile_tokens) && tok >= 0 && tok < A.T)
+                const int i = r / A.G, tok = d.tok0 + i;
+                if (i < d.tokens && tok >= 0 && tok < A.T)
                     dst = reinterpret_cast<T *>(A.out) + (long long)tok * A.o_t +
                           (long long)(d.h * A.G + r - i * A.G) * A.o_h + cb * TJ_COLS;
-                const int first = ta_range_lo(d.total, d.ge, c - 1) >= d.t0 - TA_ITEM_COST ? 2 * (c - 1) : 2 * (c - 1) + 1;
-                const long long last = d.t0 + d.nt - 1;
-                int c1 = (int)(last * d.ge / d.total);   // the CTA holding the item's last tile
-                while (c1 + 1 < d.ge && ta_range_lo(d.total, d.ge, c1 + 1) <= last) ++c1;
-                const int nc = c1 - (c - 1) + 1;
                 if (dst) {
 #pragma unroll 4
-                    for (int j = wr; j < nc; j += wpr) {
-                        const size_t s = j == 0 ? first : 2 * (c - 1 + j);
-                        const float2 st = A.stats[s * rows + r];
-                        const float4 *p = reinterpret_cast<const float4 *>(A.parts) + (s * (DP / 4) + cb * 2) * rows + r;
-                        const float4 a = p[0], b = p[rows];
+                    for (int j = wr; j < d.parts; j += wpr) {
+                        const size_t s = j == 0 ? d.first : 2 * (c - 1 + j);
+                        const float2 st = A.stats[s * TA_ROWS + r];
+                        const float4 *p = reinterpret_cast<const float4 *>(A.parts) + (s * (DP / 4) + cb * 2) * TA_ROWS + r;
+                        const float4 a = p[0], b = p[TA_ROWS];
                         const float v[TJ_COLS] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
                         const float mn = fmaxf(m, st.x), mz = mn == -INFINITY ? 0.0f : mn;
                         const float f = ta_exp2(m - mz), w = ta_exp2(st.x - mz);
@@ -1134,9 +1147,9 @@ static bool ta_q_map(CUtensorMap *m, const void *base, int D, int Hq, int T, lon
 }
 
 static int ta_tile_tokens(int G) { return TA_ROWS / G; }
-static int ta_part_rows(int max_new, int G) { return (max_new < ta_tile_tokens(G) ? max_new : ta_tile_tokens(G)) * G; }
+static int ta_rows(int max_new, int G) { return (max_new < ta_tile_tokens(G) ? max_new : ta_tile_tokens(G)) * G; }
 static size_t ta_desc_bytes(int grid) { return ((size_t)grid * sizeof(TaDesc) + 255) & ~(size_t)255; }
-static size_t ta_stats_bytes(int grid, int rows) { return ((size_t)2 * grid * rows * sizeof(float2) + 255) & ~(size_t)255; }
+static size_t ta_stats_bytes(int grid) { return (size_t)2 * grid * TA_ROWS * sizeof(float2); }
 
 template <typename T, int NCH, int REP>
 static int launch_ta(const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mq, TaArgs A, cudaStream_t s) {
@@ -1146,7 +1159,7 @@ static int launch_ta(const CUtensorMap &mk, const CUtensorMap &mv, const CUtenso
     const int fixed = 1024 + TA_BARS + Lay::Q_BYTES;
     int slots = (max_smem_optin(dev) - fixed) / Lay::SLOT;
     if (slots > 12) slots = 12;
-    if (slots < 4) return VT_EARG;
+    if (slots < 4 || (REP > 1 && slots * Lay::SLOT < TA_ROWS * (Lay::DP + 4) * 4)) return VT_EARG;
     A.k_slots = (slots + 1) / 2;
     A.v_slots = slots / 2;
     A.cs = A.fold ? 1024 : Lay::TK * 128;
@@ -1189,8 +1202,8 @@ extern "C" {
 
 size_t vt_tree_attention_ws_bytes(int max_new, int Hq, int Hkv, int D) {
     if (max_new < 1 || max_new > TA_MAX_NEW || Hkv < 1 || Hq < Hkv || Hq / Hkv > TA_ROWS || D < 1 || D > 256) return 0;
-    const int grid = num_sms(cur_device()), rows = ta_part_rows(max_new, Hq / Hkv), dp = (D + 63) / 64 * 64;
-    return ta_desc_bytes(grid) + ta_stats_bytes(grid, rows) + (size_t)2 * grid * rows * dp * sizeof(float);
+    const int grid = num_sms(cur_device()), dp = (D + 63) / 64 * 64;
+    return ta_desc_bytes(grid) + ta_stats_bytes(grid) + (size_t)2 * grid * TA_ROWS * dp * sizeof(float);
 }
 
 int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, void *out, const long long *strides,
@@ -1254,13 +1267,13 @@ int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, v
     if (A.o_vec && ((uintptr_t)out & 31) == 0 && ((A.o_t | A.o_h) & 15) == 0) A.o_vec = 2;
     A.negate = scale < 0.0f;
     A.sl2 = fmaxf(fabsf(scale) * 1.4426950408889634f, 1.2e-38f);   // above 0: a hidden key's -inf stays -inf
-    A.part_rows = ta_part_rows(max_new, A.G);
+    A.rows = ta_rows(max_new, A.G);
     A.timeout_ns = pipe_timeout_ns();
     const int grid = num_sms(cur_device());
     char *ws = (char *)workspace;
     A.desc = (TaDesc *)ws;
     A.stats = (float2 *)(ws + ta_desc_bytes(grid));
-    A.parts = (float *)(ws + ta_desc_bytes(grid) + ta_stats_bytes(grid, A.part_rows));
+    A.parts = (float *)(ws + ta_desc_bytes(grid) + ta_stats_bytes(grid));
     if (dtype == 0) return dispatch_ta<__half>(mk, mv, mq, A, s);
     return dispatch_ta<__nv_bfloat16>(mk, mv, mq, A, s);
 }

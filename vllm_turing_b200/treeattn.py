@@ -13,11 +13,11 @@ MAX_GROUP = 128   # query heads to a cached head
 
 _STRIDES = ctypes.c_longlong * 10
 _CODE = {torch.float16: 0, torch.bfloat16: 1}
-_ws_words = {}   # (device, rows a cached head has at most, D) -> workspace, in 32-bit words
+_ws_words = {}   # (device, D) -> workspace, in 32-bit words
 
 
 def _workspace(index, max_new, Hq, Hkv, D):
-    key = (index, max_new * Hq // Hkv, D)
+    key = (index, D)
     n = _ws_words.get(key)
     if n is None:
         with torch.cuda.device(index):
