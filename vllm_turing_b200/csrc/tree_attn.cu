@@ -21,10 +21,11 @@
 //   REP = 4 or 2 (at most 32 or 64 rows): the rows are repeated in every 128 / REP lanes, and replica p takes only the
 //     keys [p, p + 1) TK / REP of each tile (its P is zero elsewhere). Each replica has its own m, l and O; they are
 //     joined when the item ends.
-//   CH = 2 (more rows, D <= 128): two groups of four warps take the even and the odd tiles, each with its own O, so
-//     that one group's softmax runs while the other's products do.
-//   CH = 1, REP = 1 (more rows, D > 128): O fills tensor memory; one group.
-// Q is the A operand: in tensor memory (CH = 1; leaves more shared memory to the ring of K and V tiles) or shared.
+//   REP = 1 (more rows): two groups of four warps, GR = 2, take half the keys of each tile for the same rows; the two
+//     threads of a row agree on its m through shared memory.
+// Q is the A operand: in tensor memory where that leaves room beside O, S and (over S) P, which also leaves more shared
+// memory to the rings; for REP = 1 and D <= 128, where the products bound, P has columns of its own instead, so that the
+// score MMA need not wait for the P V MMA two tiles before it, and Q is in shared memory.
 //
 // Work: the key tiles of all (request, cached head, row tile) items form one line of units; each CTA (one per SM) takes
 // an equal contiguous range (computed from the lengths on the device, so a captured graph follows them), whatever
@@ -47,16 +48,17 @@ namespace vt {
 
 constexpr int TA_MAX_NEW = 64;
 constexpr int TA_ROWS = 128;
-constexpr int TA_BARS = 2048;        // barriers and small shared state, bytes
 constexpr int TA_ITEM_COST = 2;      // what an item costs besides its tiles, in tiles, when the ranges are cut
 constexpr float TA_RAISE = 8.0f;     // log2 of the factor by which weights may pass the running maximum
+
+constexpr int MAX_SLOTS = 12;        // of the K and V rings together
 
 template <int NCH, int REP> struct TaLayout {        // NCH: 64-value chunks of the head
     static constexpr int TK = NCH <= 2 ? 128 : 64;   // keys a tile: 16 .. 32 KB of K
     static constexpr int DP = NCH * 64;
-    static constexpr int CH = REP == 1 && NCH <= 2 ? 2 : 1;
-    static constexpr bool QT = CH == 1;                            // Q in tensor memory
-    static constexpr int THREADS = 128 * CH + 128;                 // rows, then the K, MMA, V and Q warps
+    static constexpr int GR = REP == 1 ? 2 : 1;                    // groups of row warps
+    static constexpr bool QT = !(REP == 1 && NCH <= 2);            // Q in tensor memory, P over S
+    static constexpr int THREADS = 128 * GR + 128;                 // rows, then the K, MMA, V and Q warps
     static constexpr int RR = TA_ROWS / REP;                       // rows of an item
     // QT: the next item's Q waits in shared memory, QC chunks of its rows at a time in QB buffers, for the row warps to
     // copy; with replicas the buffer also stages their sums when an item ends. Otherwise Q is the MMA's operand there.
@@ -69,8 +71,11 @@ template <int NCH, int REP> struct TaLayout {        // NCH: 64-value chunks of 
     // entries of the rings of segments and of "pages that are not there" words: more than the K ring's slots (half of
     // the 7 that fit, or of 12) + 2, which is how far the K warp can be ahead of the rows
     static constexpr int RING = SLOT >= 32768 ? 8 : 16;
-    static constexpr int S_COL = CH * DP, Q_COL = S_COL + 2 * TK;  // tensor memory: O (O0 O1) | S0 S1 (P over S) | Q
-    static_assert(Q_COL + (QT ? DP / 2 : 0) <= 512, "tensor memory");
+    // barriers and small shared state, bytes (checked in the kernel)
+    static constexpr int BARS = ((2 * MAX_SLOTS + 12 + RING) * 8 + RING * 56 + 40 + GR * 1024 + (6 + RING) * 4 + 127) / 128 * 128;
+    // tensor memory: O | S0 S1 | P0 P1 or Q
+    static constexpr int S_COL = DP, Q_COL = S_COL + 2 * TK, P_COL = QT ? S_COL : Q_COL, P_LD = QT ? TK : TK / 2;
+    static_assert(Q_COL + (QT ? DP / 2 : TK) <= 512, "tensor memory");
 };
 
 struct TaArgs {
@@ -356,13 +361,13 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                      const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ TaArgs A) {
     using Lay = TaLayout<NCH, REP>;
-    constexpr int TK = Lay::TK, DP = Lay::DP, CH = Lay::CH;
-    constexpr int ROW_WARPS = 4 * CH, K_WARP = ROW_WARPS, MMA_WARP = ROW_WARPS + 1, V_WARP = ROW_WARPS + 2,
+    constexpr int TK = Lay::TK, DP = Lay::DP, GR = Lay::GR;
+    constexpr int ROW_WARPS = 4 * GR, K_WARP = ROW_WARPS, MMA_WARP = ROW_WARPS + 1, V_WARP = ROW_WARPS + 2,
                   Q_WARP = ROW_WARPS + 3;
     constexpr bool QT = Lay::QT;
     constexpr int TA_RING = Lay::RING;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    unsigned char *qs = tc_align1024(smem_raw);
+    unsigned char *qs = smem_raw;   // 1024-byte aligned (checked below): the block has no static shared memory
     const int SK = A.k_slots, SV = A.v_slots;
     unsigned char *kring = qs + Lay::Q_BYTES, *vring = kring + (size_t)SK * Lay::SLOT;
     float *stage = reinterpret_cast<float *>(qs);   // [128][STAGE_LD] (REP > 1)
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
     uint64_t *vfull = kempty + SK;
     uint64_t *vempty = vfull + SV;
     uint64_t *sfull = vempty + SV;      // [2] scores in S buffer
-    uint64_t *pfull = sfull + 2;        // [2] weights over them (and V ready for use), 4 row warps arrive
+    uint64_t *pfull = sfull + 2;        // [2] weights from them (and V ready for use), the row warps arrive
     uint64_t *pvdone = pfull + 2;       // [2] the MMAs that read them (and added to O) have completed
     uint64_t *qfull = pvdone + 2;       // [1] Q in place for the MMA (QT: the row warps arrive, else the Q warp)
     uint64_t *qbfull = qfull + 1;       // [2] QT: Q buffer loaded
@@ -380,15 +385,31 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
     uint64_t *segfull = drain + 1;      // [TA_RING]
     TaSeg *segs = reinterpret_cast<TaSeg *>(segfull + TA_RING);   // [TA_RING]
     TaPlan *plan = reinterpret_cast<TaPlan *>(segs + TA_RING);
-    float2 *ml = reinterpret_cast<float2 *>(plan + 1);            // [128] m and l of the replicas / the other group
+    float2 *ml = reinterpret_cast<float2 *>(plan + 1);            // REP > 1: [128] m and l of the replicas
+    float(*hm)[2][TA_ROWS] = reinterpret_cast<float(*)[2][TA_ROWS]>(ml);   // GR == 2: [tile & 1][group] maxima, sums
     long long *wsum = reinterpret_cast<long long *>(ml);          // [warps], before
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(ml + TA_ROWS);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(hm + (GR == 2 ? 2 : 1));
     uint32_t *wild = tmem_slot + 1;                               // [2 segments][2 words]
     volatile uint32_t *more = wild + 4;                           // [1] the rows have another segment
     volatile uint32_t *bad = wild + 5;                            // [TA_RING] 8-row groups not there
+    // what stands between kfull and here, at the most slots, fits the bytes that the host adds to Q and the rings
+    static_assert(sizeof(TaSeg) == 56 && sizeof(TaPlan) == 40 &&
+                      8 * (2 * MAX_SLOTS + 2 + 2 + 2 + 1 + 2 + 2 + 1 + TA_RING) + TA_RING * (int)sizeof(TaSeg) +
+                              (int)sizeof(TaPlan) + GR * 2 * TA_ROWS * 4 + 4 * (1 + 4 + 1 + TA_RING) <=
+                          Lay::BARS,
+                  "shared state");
+    static_assert(Lay::THREADS / 32 * 8 <= GR * 2 * TA_ROWS * 4, "sums of the plan");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
+    if (smem_u32(smem_raw) & 1023u) {   // the tiles' swizzle needs it
+        pdl_wait();
+        if (threadIdx.x == 0) {
+            A.desc[blockIdx.x].split = 0;
+            report(A.status, ST_PIPE_TIMEOUT | 0x2f0u);
+        }
+        return;
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < SK; ++s) {
             mbar_init(&kfull[s], 1);
@@ -401,7 +422,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         for (int s = 0; s < TA_RING; ++s) mbar_init(&segfull[s], 1);
         for (int b = 0; b < 2; ++b) {
             mbar_init(&sfull[b], 1);
-            mbar_init(&pfull[b], 4);
+            mbar_init(&pfull[b], ROW_WARPS);
             mbar_init(&pvdone[b], 1);
             mbar_init(&qbfull[b], 1);
             mbar_init(&qbempty[b], QT ? ROW_WARPS : 1);
@@ -520,7 +541,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         };
         auto scores = [&](int gt) {   // S[gt] = Q K^T of the next K tile
             if (!wait(&kfull[ks], kphase, 0x220u)) return false;
-            if (gt > 1 && !wait(&pvdone[gt & 1], ((uint32_t)(gt >> 1) & 1u) ^ 1u, 0x228u)) return false;   // P over S
+            if (QT && gt > 1 && !wait(&pvdone[gt & 1], ((uint32_t)(gt >> 1) & 1u) ^ 1u, 0x228u)) return false;   // P over S
             const uint64_t kd = ta_k_desc(kring0 + (uint32_t)(ks * Lay::SLOT), A.gs);
             const uint32_t d = tb + Lay::S_COL + (uint32_t)((gt & 1) * TK);
 #pragma unroll
@@ -545,12 +566,11 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                 ok = ok && wait(&pfull[g & 1], (uint32_t)(g >> 1) & 1u, 0x240u);
                 ok = ok && wait(&vfull[vs], vphase, 0x250u);
                 if (!ok) break;
-                const uint32_t o = tb + (CH == 2 ? (uint32_t)((g & 1) * DP) : 0u);
-                const uint32_t p = tb + Lay::S_COL + (uint32_t)((g & 1) * TK);
+                const uint32_t p = tb + Lay::P_COL + (uint32_t)((g & 1) * Lay::P_LD);
                 const uint64_t v = ta_v_desc(vring0 + (uint32_t)(vs * Lay::SLOT), A.cs, A.gs);
 #pragma unroll
                 for (int i = 0; i < TK / 16; ++i)   // 16 keys a step: 8 columns of P, two groups of rows of V
-                    umma_f16_ts_e(o, p + 8 * i, v + (uint64_t)(i * (A.gs >> 3)), id_o, (t >= CH || i > 0) ? 1u : 0u);
+                    umma_f16_ts_e(tb, p + 8 * i, v + (uint64_t)(i * (A.gs >> 3)), id_o, (t > 0 || i > 0) ? 1u : 0u);
                 umma_commit_e(&pvdone[g & 1]);
                 umma_commit_e(&vempty[vs]);
                 if (++vs == SV) vs = 0, vphase ^= 1u;
@@ -603,8 +623,8 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         // ---------------- rows: softmax and output ----------------
         const int q4 = warp & 3, grp = warp >> 2;
         const int tid = q4 * 32 + lane;             // lane of tensor memory this thread holds
-        constexpr int RR = TA_ROWS / REP, CPT = TK / REP;   // rows; keys of a tile a thread takes
-        const int row = tid % RR, part = tid / RR;
+        constexpr int RR = TA_ROWS / REP, CPT = TK / REP / GR;   // rows; keys of a tile a thread takes
+        const int row = tid % RR, part = GR == 2 ? grp : tid / RR;
         const uint32_t lane_base = tmem_base + ((uint32_t)(q4 * 32) << 16);
         bool dead = false;
         auto wait = [&](uint64_t *bar, uint32_t parity, unsigned code) {
@@ -620,7 +640,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         auto open = [&]() {
             wait(&segfull[seg % TA_RING], (uint32_t)(seg / TA_RING) & 1u, 0x258u);
             if (threadIdx.x == 0) *more = !dead && segs[seg % TA_RING].tiles != 0;   // one thread decides: the warps'
-            named_sync(TC_EPI_BAR, 128 * CH);                                        // barriers must match
+            named_sync(TC_EPI_BAR, 128 * GR);                                        // barriers must match
             if (!*more) return false;
             if constexpr (QT) {
                 constexpr int QC = Lay::QC, QB = Lay::QB;
@@ -631,6 +651,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                     const unsigned char *buf = qs + b * Lay::Q_ROUND + row * 128;
 #pragma unroll
                     for (int c = 0; c < QC && c0 + c < NCH; ++c) {   // rows past the item's hold anything
+                        if (GR == 2 && ((c0 + c) & 1) != grp) continue;
                         uint32_t w[32];
 #pragma unroll
                         for (int v = 0; v < 8; ++v) {
@@ -672,7 +693,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         }
         while (has) {
             const TaSeg &sg = segs[seg % TA_RING];
-            const int N = sg.tiles, L = sg.L, ctx = L - sg.n, kt0 = sg.kt0, g0 = g;
+            const int N = sg.tiles, L = sg.L, ctx = L - sg.n, kt0 = sg.kt0;
             const int live = min(min(sg.n, A.max_new) - sg.rt * A.tile_tokens, A.tile_tokens) * A.G;
             const int row_i = row / A.G, tok_i = sg.rt * A.tile_tokens + row_i, tok = sg.cu0 + tok_i;
             const bool mine = row < live && tok >= 0 && tok < A.T;
@@ -685,90 +706,74 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             float m = -INFINITY, l = 0.0f;
             for (int t = 0; t < N; ++t, ++g) {
                 const int buf = g & 1;
-                if (CH == 2 && buf != grp) continue;
                 const int k0 = (kt0 + t) * TK;
                 const uint32_t use = (uint32_t)(g >> 1);
                 const bool past = k0 + TK > ctx;
                 const uint32_t s_col = lane_base + Lay::S_COL + (uint32_t)(buf * TK);
+                const uint32_t p_col = lane_base + Lay::P_COL + (uint32_t)(buf * Lay::P_LD);
                 wait(&sfull[buf], use & 1u, 0x260u);
                 const uint32_t gone = bad[g % TA_RING];
                 if (warp_live) {
-                    // W keys at a time; a thread with more (CH = 2, which leaves it 168 registers) reads its scores
-                    // twice, a chunk ahead of the one it works on
-                    constexpr int W = CH == 2 ? 32 : CPT, LD = CPT < 32 ? CPT : 32, NW = CPT / W;
-                    float x[NW > 1 ? 2 : 1][W < 32 ? 32 : W];
-                    auto fetch = [&](int i, int n) {
+                    constexpr int LD = CPT < 32 ? CPT : 32;
+                    float x[CPT < 32 ? 32 : CPT];
 #pragma unroll
-                        for (int c = 0; c < W; c += LD)
-                            ta_ld<LD>(s_col + (uint32_t)(part * CPT + n * W + c), reinterpret_cast<uint32_t *>(&x[i][c]));
-                    };
-                    auto hide = [&](int i, int n) {
-                        if (past || gone != 0) {
+                    for (int c = 0; c < CPT; c += LD)
+                        ta_ld<LD>(s_col + (uint32_t)(part * CPT + c), reinterpret_cast<uint32_t *>(&x[c]));
+                    tmem_ld_wait();
+                    if (past || gone != 0) {
 #pragma unroll
-                            for (int c = 0; c < W; c += LD) {
-                                const int kk = part * CPT + n * W + c;
-                                uint32_t vis = ta_seen(see, k0 + kk, ctx);
-                                const uint32_t g4 = (gone >> (kk / 8)) & 15u;
-                                vis &= ~(((g4 * 0x00204081u) & 0x01010101u) * 255u);
+                        for (int c = 0; c < CPT; c += LD) {
+                            const int kk = part * CPT + c;
+                            uint32_t vis = ta_seen(see, k0 + kk, ctx);
+                            const uint32_t g4 = (gone >> (kk / 8)) & 15u;
+                            vis &= ~(((g4 * 0x00204081u) & 0x01010101u) * 255u);
 #pragma unroll
-                                for (int j = 0; j < LD; ++j) x[i][c + j] = (vis >> j) & 1u ? x[i][c + j] : -INFINITY;
-                            }
+                            for (int j = 0; j < LD; ++j) x[c + j] = (vis >> j) & 1u ? x[c + j] : -INFINITY;
                         }
-                    };
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    fetch(0, 0);
-#pragma unroll
-                    for (int n = 0; n < NW; ++n) {
-                        const int i = NW > 1 ? n & 1 : 0;
-                        tmem_ld_wait();
-                        if (NW > 1) fetch(i ^ 1, (n + 1) % NW);
-                        hide(i, n);
-#pragma unroll
-                        for (int j = 0; j < W; ++j) mx[j & 3] = fmaxf(mx[j & 3], x[i][j]);
                     }
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int j = 0; j < CPT; ++j) mx[j & 3] = fmaxf(mx[j & 3], x[j]);
+                    float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    if (GR == 2) {   // the two warps that hold these rows (and have read their scores: P may go over them)
+                        hm[buf][grp][row] = top;
+                        named_sync(TC_EPI_BAR + 1 + q4, 64);
+                        top = fmaxf(top, hm[buf][grp ^ 1][row]);
+                    }
                     const float tm = top * A.sl2;   // sl2 > 0
                     const bool raise = tm > m + TA_RAISE || (m == -INFINITY && tm > m);
                     if (__any_sync(0xffffffffu, raise)) {
                         const float f = raise ? ta_exp2(m - tm) : 1.0f;
                         if (raise) m = tm;
                         l *= f;
-                        if (t >= CH) {   // O of the tiles before this one
-                            if (CH == 1) wait(&pvdone[(g - 1) & 1], (uint32_t)((g - 1) >> 1) & 1u, 0x270u);
+                        if (t > 0) {   // O of the tiles before this one; a group's share of its columns
+                            wait(&pvdone[(g - 1) & 1], (uint32_t)((g - 1) >> 1) & 1u, 0x270u);
 #pragma unroll 1
-                            for (int c = 0; c < DP; c += 32) {
+                            for (int c = grp * (DP / GR); c < (grp + 1) * (DP / GR); c += 32) {
                                 uint32_t o[32];
-                                tmem_ld32(lane_base + (uint32_t)(grp * DP + c), o);
+                                tmem_ld32(lane_base + (uint32_t)c, o);
                                 tmem_ld_wait();
 #pragma unroll
                                 for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                                tmem_st32(lane_base + (uint32_t)(grp * DP + c), o);
+                                tmem_st32(lane_base + (uint32_t)c, o);
                             }
                         }
                     }
                     constexpr float BIAS = std::is_same<T, __half>::value ? 7.0f : 0.0f;
                     const float off = (m == -INFINITY ? 0.0f : -m) + BIAS;
                     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    uint32_t w[W / 2];
+                    uint32_t w[CPT / 2];
 #pragma unroll
-                    for (int n = 0; n < NW; ++n) {
-                        const int i = NW > 1 ? n & 1 : 0;
-                        if (NW > 1) {
-                            tmem_ld_wait();
-                            if (n + 1 < NW) fetch(i ^ 1, n + 1);
-                            hide(i, n);
-                        }
-#pragma unroll
-                        for (int j = 0; j < W; j += 2) {   // a hidden key: 2^-inf = 0
-                            const float a = ta_exp2(__fmaf_rn(x[i][j], A.sl2, off));
-                            const float b = ta_exp2(__fmaf_rn(x[i][j + 1], A.sl2, off));
-                            sum[j & 2] += a;
-                            sum[(j & 2) + 1] += b;
-                            w[j >> 1] = ta_pack<T>(a, b);
-                        }
-                        // over scores already read: key k's column of P is k / 2
-                        if constexpr (REP == 1) ta_st<W / 2>(s_col + (uint32_t)(n * W / 2), w);
+                    for (int j = 0; j < CPT; j += 2) {   // a hidden key: 2^-inf = 0
+                        const float a = ta_exp2(__fmaf_rn(x[j], A.sl2, off));
+                        const float b = ta_exp2(__fmaf_rn(x[j + 1], A.sl2, off));
+                        sum[j & 2] += a;
+                        sum[(j & 2) + 1] += b;
+                        w[j >> 1] = ta_pack<T>(a, b);
                     }
+                    if (!QT && g > 1)   // the MMAs that read this P buffer two tiles ago
+                        wait(&pvdone[buf], (use & 1u) ^ 1u, 0x280u);
+                    if constexpr (REP == 1) ta_st<CPT / 2>(p_col + (uint32_t)(part * (CPT / 2)), w);
                     if constexpr (REP > 1) {
                         // the replica's CPT / 2 columns of P, zeros in the others'
 #pragma unroll
@@ -777,7 +782,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
                                 z[j] = (c + j) / (CPT / 2) == part ? w[j % (CPT / 2)] : 0u;
-                            ta_st<32>(s_col + (uint32_t)c, z);
+                            ta_st<32>(p_col + (uint32_t)c, z);
                         }
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -788,7 +793,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                     const int r0 = max(ctx - k0, 0);
                     wait(&vfull[g % SV], (uint32_t)(g / SV) & 1u, 0x290u);
                     unsigned char *vs = vring + (size_t)(g % SV) * Lay::SLOT;
-                    for (int idx = tid; idx < (TK - r0) * NCH * 8 && !dead; idx += 128) {
+                    for (int idx = threadIdx.x; idx < (TK - r0) * NCH * 8 && !dead; idx += 128 * GR) {
                         const int r = r0 + idx / (NCH * 8), v = idx % (NCH * 8), j = k0 + r;
                         uint4 *p = reinterpret_cast<uint4 *>(vs + (r >> 3) * A.gs + (v >> 3) * A.cs + (r & 7) * 128 +
                                                              (((v & 7) ^ (r & 7)) << 4));
@@ -820,29 +825,17 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             ++seg;
             has = open();
             wait(&pvdone[(g - 1) & 1], (uint32_t)((g - 1) >> 1) & 1u, 0x2a0u);
-            if (CH == 2 && N > 1) wait(&pvdone[g & 1], (uint32_t)((g - 2) >> 1) & 1u, 0x2a8u);
             if (threadIdx.x == 0) {   // the words of the segment after this one
                 wild[(seg & 1) * 2] = 0;
                 wild[(seg & 1) * 2 + 1] = 0;
             }
-            // join the replicas' or the two groups' sums: a factor for each, and the common m and l
-            float f0 = 1.0f, f1 = 0.0f;
-            if constexpr (CH == 2) {
-                // group 0's over, then group 1's back (a thread reads the word before it writes it)
-                float2 a = make_float2(m, l), b = a;
-                if (grp == 0) ml[tid] = a;
+            // the sums of the replicas or of the two groups: a factor for the replica's, and the common m and l
+            float f0 = 1.0f;
+            if constexpr (GR == 2) {
+                float *mine2 = hm[(g - 1) & 1][grp];   // the last tile's maxima have been read
+                mine2[row] = l;
                 named_sync(TC_EPI_BAR, 256);
-                if (grp == 1) {
-                    a = ml[tid];
-                    ml[tid] = b;
-                }
-                named_sync(TC_EPI_BAR, 256);
-                if (grp == 0) b = ml[tid];
-                m = fmaxf(a.x, b.x);
-                const float mz = m == -INFINITY ? 0.0f : m;
-                f0 = ta_exp2(a.x - mz);
-                f1 = ta_exp2(b.x - mz);
-                l = f0 * a.y + f1 * b.y;
+                l = hm[(g - 1) & 1][0][row] + hm[(g - 1) & 1][1][row];
             } else if constexpr (REP > 1) {
                 ml[tid] = make_float2(m, l);
                 named_sync(TC_EPI_BAR, 128);
@@ -857,8 +850,6 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                     l += ta_exp2(o.x - mz) * o.y;
                 }
                 f0 = ta_exp2(m0 - mz);
-            } else {
-                named_sync(TC_EPI_BAR, 128);
             }
             const volatile uint32_t *wv = wild + ((seg & 1) ^ 1) * 2;
             const unsigned long long wn = see & (wv[0] | (unsigned long long)wv[1] << 32);
@@ -962,23 +953,12 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                 }
               if (!whole && mine && part == 0) A.stats[slot * TA_ROWS + row] = make_float2(m, l);
             } else if (warp_live) {
-                constexpr int HALF = CH == 2 ? DP / 2 : DP;   // a group's share of the columns
+                constexpr int SHARE = DP / GR;   // a group's share of the columns
 #pragma unroll 1
-                for (int c = grp * HALF; c < (grp + 1) * HALF; c += 32) {
+                for (int c = grp * SHARE; c < (grp + 1) * SHARE; c += 32) {
                     float o[32];
-                    if constexpr (CH == 2) {
-                        const bool has0 = N > 1 || (g0 & 1) == 0, has1 = N > 1 || (g0 & 1) == 1;
-                        float y[32];
-                        if (has0) tmem_ld32(lane_base + (uint32_t)c, *reinterpret_cast<uint32_t(*)[32]>(o));
-                        if (has1) tmem_ld32(lane_base + (uint32_t)(DP + c), *reinterpret_cast<uint32_t(*)[32]>(y));
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            o[e] = (has0 && f0 != 0.0f ? o[e] * f0 : 0.0f) + (has1 && f1 != 0.0f ? y[e] * f1 : 0.0f);
-                    } else {
-                        tmem_ld32(lane_base + (uint32_t)c, *reinterpret_cast<uint32_t(*)[32]>(o));
-                        tmem_ld_wait();
-                    }
+                    tmem_ld32(lane_base + (uint32_t)c, *reinterpret_cast<uint32_t(*)[32]>(o));
+                    tmem_ld_wait();
                     if (mine && !dead) put(o, c);
                 }
                 if (!whole && mine && grp == 0) A.stats[slot * TA_ROWS + row] = make_float2(m, l);
@@ -988,7 +968,6 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                 if (has && lane == 0) mbar_arrive(&qbempty[0]);
             }
             tc_fence_before();
-            if (CH == 2) named_sync(TC_EPI_BAR, 256);   // both groups have read both O
         }
     }
     // all roles done: free TMEM after every TMEM access and MMA of the CTA has completed
@@ -1156,9 +1135,9 @@ static int launch_ta(const CUtensorMap &mk, const CUtensorMap &mv, const CUtenso
     using Lay = TaLayout<NCH, REP>;
     const int dev = cur_device();
     if (dev < 0 || dev >= VT_MAX_DEV) return VT_EARG;
-    const int fixed = 1024 + TA_BARS + Lay::Q_BYTES;
+    const int fixed = Lay::BARS + Lay::Q_BYTES;
     int slots = (max_smem_optin(dev) - fixed) / Lay::SLOT;
-    if (slots > 12) slots = 12;
+    if (slots > MAX_SLOTS) slots = MAX_SLOTS;
     if (slots < 4 || (REP > 1 && slots * Lay::SLOT < TA_ROWS * (Lay::DP + 4) * 4)) return VT_EARG;
     A.k_slots = (slots + 1) / 2;
     A.v_slots = slots / 2;
