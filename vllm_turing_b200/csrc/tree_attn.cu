@@ -741,7 +741,8 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                         top = fmaxf(top, hm[buf][grp ^ 1][row]);
                     }
                     const float tm = top * A.sl2;   // sl2 > 0
-                    const bool raise = tm > m + TA_RAISE || (m == -INFINITY && tm > m);
+                    // (a row that is none holds anything: it must not make its warp rescale)
+                    const bool raise = row < live && (tm > m + TA_RAISE || (m == -INFINITY && tm > m));
                     if (__any_sync(0xffffffffu, raise)) {
                         const float f = raise ? ta_exp2(m - tm) : 1.0f;
                         if (raise) m = tm;
@@ -771,8 +772,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                         sum[(j & 2) + 1] += b;
                         w[j >> 1] = ta_pack<T>(a, b);
                     }
-                    if (!QT && g > 1)   // the MMAs that read this P buffer two tiles ago
-                        wait(&pvdone[buf], (use & 1u) ^ 1u, 0x280u);
+                    // P's columns are free: sfull was committed after the MMAs that read them two tiles ago
                     if constexpr (REP == 1) ta_st<CPT / 2>(p_col + (uint32_t)(part * (CPT / 2)), w);
                     if constexpr (REP > 1) {
                         // the replica's CPT / 2 columns of P, zeros in the others'
