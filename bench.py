@@ -66,6 +66,10 @@ def parse():
     ap.add_argument("--mlp", default="unfused", choices=["fused", "unfused"],
                     help="decode: gate_up then SiLU*up + quant as the reference's two ops (scaled_mm_, silu_mul_quant; "
                          "default) or as one kernel (w8a8.gate_up_silu_quant; measured ~1 us per layer slower)")
+    ap.add_argument("--context", type=int, default=0,
+                    help="stack: run the attention of the M tokens over a paged cache of this many earlier tokens per "
+                         "layer (step tables, rotary + cache write, tree attention; M <= 64, at most 4 ranks) instead "
+                         "of its stand-in")
     ap.add_argument("--no-e2e", action="store_true")
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--profile", action="store_true", help="short run for ncu: no clocks, e2e or CPU baseline")
@@ -1001,13 +1005,54 @@ def run_p2p(args, world, rank, local, dev, gloo):
 QKV, HEADS_OUT = 14336, 6144   # the attention's input projection (q with its gate, k, v) and o_proj's K (24 x 256)
 
 
+class StackAttention:
+    """The attention of run_stack's decode step for one request: its own paged cache per layer, the tables of a step."""
+
+    def __init__(self, M, context, hq, hkv, layers, dev, block=16):
+        import torch
+
+        from vllm_turing_b200 import rotary, steptables, treeattn
+        self.rotary, self.tables, self.attn = rotary, steptables, treeattn
+        self.M, self.hq, self.hkv, self.block = M, hq, hkv, block
+        blocks = -(-(context + M) // block)
+        ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)   # noqa: E731
+        self.table, self.held = torch.full((1, blocks), -1, dtype=torch.int32, device=dev), ints([0])
+        self.free, self.count = torch.randperm(blocks, device=dev, dtype=torch.int32), ints([blocks])
+        self.cached, self.new = ints([context]), ints([M])
+        self.st = steptables.alloc_tables(1, M, False, dev)
+        self.freqs = rotary.rope_frequencies(64, 1e7, device=dev)
+        g = torch.Generator(device=dev).manual_seed(11)
+        self.caches = [[torch.empty(blocks, block, hkv, 256, dtype=torch.bfloat16, device=dev).normal_(generator=g)
+                        for _ in range(2)] for _ in range(layers)]
+        self.at = 0
+
+    def begin(self):
+        """Once per step: the tables every layer uses."""
+        self.tables.step_tables(self.table, self.held, self.free, self.count, self.cached, self.new, self.block, self.M,
+                                out=self.st)
+        self.at = 0
+
+    def layer(self, qkv):
+        """Attention output [M, hq * 256] of one layer's [q | gate | k | v] columns."""
+        M, nq, nk = self.M, self.hq * 256, self.hkv * 256
+        q, k, v = qkv[:, :nq], qkv[:, 2 * nq:2 * nq + nk], qkv[:, 2 * nq + nk:2 * nq + 2 * nk]
+        kc, vc = self.caches[self.at]
+        self.at += 1
+        q = self.rotary.rotary_cache(q.view(M, self.hq, 256), k.view(M, self.hkv, 256), v.view(M, self.hkv, 256),
+                                     self.st.positions, self.st.slots, kc, vc, self.freqs)
+        return self.attn.tree_attention(q, kc, vc, self.table, self.st.cu, self.st.seq_lens, M).view(M, nq)
+
+
 def run_stack(args, world, rank, local, dev, gloo):
     """a synthetic 64-layer W8A8 stack at N ranks through the public API, then the int8 LM head.
     Per layer (random-init weights of these shapes, each layer its own, so every step streams them from HBM):
       1. QKV, column-parallel: vllm_turing::scaled_mm_ 5120 -> 14336 / N, its output all-gathered along the last
          dimension (dmaag.all_gather_dim, the dmaag all-gather) -- the gathered output config 4 names;
-      2. attention is out of scope: its stand-in output is this rank's first 6144 / N QKV columns, quantised per token
-         (the scaled_int8_quant replacement);
+      2. attention: by default a stand-in, this rank's first 6144 / N QKV columns. With --context L the M tokens (one
+         request's drafted tokens, a chain) attend to L earlier ones and themselves: rotary_cache on this rank's 24 / N
+         query and 4 / N cached heads of 256 (a quarter of each rotated), then tree_attention over the layer's own
+         paged cache; the step's tables (step_tables) are made once per step. The output gate's columns are not used.
+         Either way the output is quantised per token (the scaled_int8_quant replacement);
       3. o_proj, row-parallel: TPComm.row_linear 6144 / N -> 5120 fused with the all-reduce, residual add, RMSNorm and
          int8 quant (decode: the one-kernel tail; prefill: the GEMM with the reduce-scatter in its epilogue + tail);
       4. gate_up 5120 -> 34816 / N + silu_mul_quant, down 17408 / N -> 5120 fused like o_proj; its int8 output is the
@@ -1065,12 +1110,16 @@ def run_stack(args, world, rank, local, dev, gloo):
     w8a8.workspace(dev, M, max(n_qkv, n_gu))
     lmhead.workspace(dev, HIDDEN)
     stream = torch.cuda.current_stream()
+    att = None
+    if args.context > 0:
+        assert M <= 64 and 4 % world == 0, "--context: at most 64 tokens and 4 ranks"
+        att = StackAttention(M, args.context, 24 // world, 4 // world, NL, dev)
 
     def layer(s):
         torch.ops.vllm_turing.scaled_mm_(qkv_out, x_q, s["qkv_w"].t(), x_s, s["qkv_sw"], None)
         if world > 1:
             dmaag.all_gather_dim(comm, qkv_out, -1)   # column-parallel output, gathered (config 4)
-        a_q, a_s = scaled_int8_quant_cuda(qkv_out[:, :k_o])   # the attention output's stand-in
+        a_q, a_s = scaled_int8_quant_cuda(att.layer(qkv_out) if att else qkv_out[:, :k_o])
         comm.row_linear(a_q, s["o_w"], a_s, s["o_sw"], residual=residual, norm_w=norm_w, eps=1e-6, q=x_q, scales=x_s)
         torch.ops.vllm_turing.scaled_mm_(out_gu, x_q, s["gu_w"].t(), x_s, s["gu_sw"], None)
         silu_mul_quant(out_gu, h_q, h_s)
@@ -1080,6 +1129,8 @@ def run_stack(args, world, rank, local, dev, gloo):
         lmhead.logits_gathered(residual[M - m_head:], head_w, head_s, comm=comm if world > 1 else None, out=logits)
 
     def step():
+        if att:
+            att.begin()
         for s in layers:
             layer(s)
         head()
@@ -1182,7 +1233,7 @@ def run_stack(args, world, rank, local, dev, gloo):
                                f"o_proj 6144->5120 and down 17408->5120 (row-parallel, fused all-reduce + residual + "
                                f"RMSNorm + int8 quant), gate_up 5120->34816 + SiLU*up + quant; int8 LM head "
                                f"5120->151936 on {m_head} row(s), logits all-gathered; M={M}",
-                   "tokens": M, "layers": NL, "tp": world, "head_rows": m_head,
+                   "tokens": M, "layers": NL, "tp": world, "head_rows": m_head, "context": args.context,
                    "l2": f"inputs larger than L2: {NL} layers with their own weights",
                    "launch": "CUDA graph of the step, replayed K times", "parallelism": f"tp{world}"},
         "clocks": clk.summary(), "e2e": e2e, "cpu_baseline": None, "parity": parity,

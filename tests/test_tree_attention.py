@@ -374,3 +374,58 @@ def test_refusals():
     for bad in (dict(q=b(3, 4, 64).float()), dict(v_cache=b(2, 16, 2, 64).half()), dict(out=b(3, 4, 64).half())):
         with pytest.raises(TypeError):
             A.tree_attention(**{**good, **bad})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("G", [1, 8, 20], ids=["32 rows", "64 rows", "more"])
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+def test_every_kernel(D, G):
+    """Each head size with few and many rows: other scales, several row tiles, a long context that is cut into parts,
+    and what a row may not see, wild values in the step's own rows among it."""
+    n = 8 if G > 1 else 16
+    c = make([n + 3, 700, 9000], [n, n, n], G, 1, D, 16, torch.bfloat16, seed=G, trees=True)
+    check(c, run(c))
+    for scale in (0.0, -0.2, 0.5):
+        check(c, run(c, scale=scale), scale=scale)
+    words = c["mask"].tolist()
+    for b, L in enumerate((n + 3, 700, 9000)):
+        hidden = [i for i in range(n) if all(i == t or not (words[b * n + t] >> i) & 1 for t in range(n))]
+        for i in hidden[:2]:   # leaves: only their own row sees them
+            for what, (cache, x) in enumerate(zip((c["kc"], c["vc"]), c["keys"][b])):
+                if what:
+                    x[L - n + i, 0, i % D] = float("nan") if i % 2 else float("inf")
+                    x[L - n + i, 0, D - 1] = -float("inf")
+                    j = L - n + i
+                    cache[c["table"][b, j // 16].long(), j % 16] = x[j]
+    check(c, run(c))
+
+
+@pytest.mark.gpu
+def test_shared_blocks_and_empty_calls():
+    """Requests that share a prefix's blocks; no tokens; no requests."""
+    c = make([160, 0], [4, 0], 6, 2, 128, 16, torch.bfloat16, seed=11)
+    d = make([160, 170], [4, 4], 6, 2, 128, 16, torch.bfloat16, seed=11)
+    d["table"][1, :9] = d["table"][0, :9]   # 144 keys of the first request
+    for i in range(2):
+        d["keys"][1][i][:144] = d["keys"][0][i][:144]
+    check(d, run(d))
+    empty = c["q"][:0]
+    assert A.tree_attention(empty, c["kc"], c["vc"], c["table"], c["cu"], c["lens"], 4).shape == empty.shape
+    z = torch.zeros(0, 3, dtype=torch.int32, device="cuda")
+    out = torch.full_like(c["q"], 3.0)
+    A.tree_attention(c["q"], c["kc"], c["vc"], z, z.new_zeros(1), z[:, 0].contiguous(), 4, out=out)
+    assert (out == 3).all()
+
+
+@pytest.mark.gpu
+def test_context_values_that_are_not_finite():
+    """An infinity or NaN in the context is seen by every row of its head: the rows it reaches are not finite."""
+    for Hq, D in ((2, 64), (40, 128), (8, 256)):
+        c = make([300], [3], Hq, 2, D, 16, torch.bfloat16, seed=2)
+        page = c["table"][0].long()
+        c["vc"][page[100 // 16], 100 % 16, 0, 5] = float("inf")
+        out = run(c)
+        assert not torch.isfinite(out[:, :Hq // 2, 5]).any()
+        assert torch.isfinite(out[:, Hq // 2:]).all() and torch.isfinite(out[:, :Hq // 2, 6]).all()
+        c["kc"][page[200 // 16], 200 % 16, 1] = float("nan")
+        assert run(c)[:, Hq // 2:].isnan().all()

@@ -1,0 +1,121 @@
+"""The step tables, the rotary cache write and the tree attention run together, as a decode loop with drafted trees runs
+them, against a model that keeps no cache: each step drafts a tree, verifies it over the paged cache, accepts a path,
+moves its rows to the front of the tree's slots and goes on from there."""
+import math
+
+import pytest
+import torch
+
+from vllm_turing_b200 import rotary as R
+from vllm_turing_b200 import steptables as S
+from vllm_turing_b200 import treeattn as A
+from vllm_turing_b200.quantfuse import scaled_int8_quant_cuda
+
+HQ, HKV, D, ROT, BS = 6, 2, 128, 32, 16
+DT = torch.bfloat16
+
+
+def rotated(x, pos, turns):
+    """The rotation in 64 bits, rounded to the cache's type as the kernel's result is."""
+    a = pos.double()[:, None, None] * (turns * 2 * math.pi)
+    y = x.double().clone()
+    x1, x2 = x.double()[..., :ROT // 2], x.double()[..., ROT // 2:ROT]
+    y[..., :ROT // 2], y[..., ROT // 2:ROT] = x1 * a.cos() - x2 * a.sin(), x2 * a.cos() + x1 * a.sin()
+    return y.to(DT)
+
+
+def attend(q, k, v):
+    """One token's attention over its keys in 64 bits, and the bound of the kernel's error (see test_tree_attention)."""
+    G = HQ // HKV
+    kk, vv, qq = k.double().repeat_interleave(G, 1), v.double().repeat_interleave(G, 1), q.double()
+    s = torch.einsum("hd,jhd->hj", qq, kk) * D ** -0.5
+    p = torch.softmax(s, -1)
+    o, a = torch.einsum("hj,jhd->hd", p, vv), torch.einsum("hj,jhd->hd", p, vv.abs())
+    mag = (torch.einsum("hd,jhd->hj", qq.abs(), kk.abs()) * D ** -0.5).amax(-1)
+    h = torch.finfo(DT).eps / 2
+    d = (2 * D * 2.0 ** -24 * mag + 2.0 ** -21)[:, None]
+    # a rotated q or k may round to its neighbour: eps of each, which moves a score by 2 eps mag and a weight, and the
+    # sum of the weights, by that
+    d = d + 2 * torch.finfo(DT).eps * mag[:, None]
+    return o, h * o.abs() + (h + 2 * torch.expm1(d) + 2 * len(k) * 2.0 ** -24) * a * (1 + h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graph", [False, True])
+def test_tree_decoding(graph):
+    g = torch.Generator().manual_seed(5)
+    dev, B, steps, most = "cuda", 3, 6, 7
+    T = B * most
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)   # noqa: E731
+    blocks = 40
+    table, held = torch.full((B, 12), -1, dtype=torch.int32, device=dev), ints([0] * B)
+    free, count = torch.randperm(blocks, generator=g).to(torch.int32).to(dev), ints([blocks])
+    kc, vc = [torch.full((blocks, BS, HKV, D), float("nan"), dtype=DT, device=dev) for _ in range(2)]
+    f = R.rope_frequencies(ROT, 10000.0, device=dev)
+    cached, new, par = ints([0] * B), ints([0] * B), ints([-1] * T)
+    st = S.alloc_tables(B, T, True, torch.device(dev))
+    q, k, v = [torch.zeros(T, h, D, dtype=DT, device=dev) for h in (HQ, HKV, HKV)]
+    out = torch.zeros_like(q)
+
+    def one_step():
+        S.step_tables(table, held, free, count, cached, new, BS, T, par, st)
+        qr = R.rotary_cache(q, k, v, st.positions, st.slots, kc, vc, f)
+        A.tree_attention(qr, kc, vc, table, st.cu, st.seq_lens, most, mask=st.mask, out=out)
+        return scaled_int8_quant_cuda(out.view(T, HQ * D))
+
+    one_step()   # no tokens: sizes what a captured step needs
+    if graph:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            quant = one_step()
+    past = [([], []) for _ in range(B)]   # accepted (rotated keys, values) of each request
+    lens = [0] * B
+    for step in range(steps):
+        n = [int(torch.randint(1, most + 1, (1,), generator=g)) for _ in range(B)]
+        if step == 0:
+            n = [most, 3, 1]
+        parents = []
+        for x in n:
+            parents += [-1 if i == 0 else int(torch.randint(0, i, (1,), generator=g)) for i in range(x)]
+        par.copy_(ints(parents + [-1] * (T - sum(n))))
+        cached.copy_(ints(lens))
+        new.copy_(ints(n))
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=g).to(DT))
+        if graph:
+            gr.replay()
+        else:
+            quant = one_step()
+        assert st.status.item() == 0
+        t = 0
+        for b in range(B):
+            rows, pos = [], []
+            for i in range(n[b]):
+                path, x = [], i
+                while x >= 0:
+                    path.insert(0, x)
+                    x = parents[t + x]
+                rows.append(path)
+                pos.append(lens[b] + len(path) - 1)
+            pos = torch.tensor(pos, device=dev)
+            assert torch.equal(st.positions[t:t + n[b]], pos)
+            kr, qr = rotated(k[t:t + n[b]], pos, f.turns), rotated(q[t:t + n[b]], pos, f.turns)
+            vt = v[t:t + n[b]]
+            for i, path in enumerate(rows):
+                keys = torch.stack(past[b][0] + [kr[j] for j in path])
+                vals = torch.stack(past[b][1] + [vt[j] for j in path])
+                want, tol = attend(qr[i], keys, vals)
+                assert ((out[t + i].double() - want).abs() <= tol).all(), (step, b, i)
+            # accept the path to a random node: its rows go to the front of the tree's slots
+            path = rows[int(torch.randint(0, n[b], (1,), generator=g))]
+            slots = st.slots[t:t + n[b]]
+            src, dst = slots[torch.tensor(path, device=dev)], slots[:len(path)]
+            for c in (kc, vc):
+                flat = c.view(-1, HKV, D)
+                flat[dst] = flat[src]
+            past[b] = (past[b][0] + [kr[j] for j in path], past[b][1] + [vt[j].clone() for j in path])
+            lens[b] += len(path)
+            t += n[b]
+        # what o_proj takes: the quantiser's rows are those of the attention's output
+        want_q, want_s = scaled_int8_quant_cuda(out.view(T, HQ * D))
+        assert torch.equal(quant[0], want_q) and torch.equal(quant[1], want_s)
