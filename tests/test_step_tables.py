@@ -137,7 +137,8 @@ def test_against_plain(name, pad, trees):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("B, hi, bs, trees", [(256, 64, 16, True), (1025, 5, 16, False), (4096, 2, 8, True),
-                                              (33, 900, 24, False), (2, 40000, 128, False)])
+                                              (33, 900, 24, False), (2, 40000, 128, False),
+                                              (700, 64, 16, True)])
 def test_many(B, hi, bs, trees):
     g = torch.Generator().manual_seed(B)
     cached = torch.randint(0, 300, (B,), generator=g).tolist()

@@ -13,8 +13,11 @@
 // itself and each ancestor, so a walk up the parents (at most 64 steps) gives both.
 //
 // Bound by latency: a few KB to a MB moved. One block does the prefix sums and the stack (its barriers replace a
-// grid-wide one); token rows are filled by the same block while they are few (one launch), by a grid of their own
-// above TOKENS_ONE_BLOCK (the second launch overlaps the first's tail by programmatic dependent launch).
+// grid-wide one) and, with few token rows, fills those too; more rows are shared out over the blocks of one cluster,
+// which wait for the first at the cluster's barrier, so the step stays one launch, and above ROWS_CLUSTER_MAX rows over a
+// grid of their own (a second launch that overlaps the first's tail by programmatic dependent launch). On the device,
+// 8300 rows of 256 trees: 8.2 us with the cluster, 7.0 us with the grid, but 20.5 against 23.4 us a call from the host;
+// 67000 rows of 64 prompts: 11.9 and 5.9 us.
 #include <limits.h>
 
 #include "common.cuh"
@@ -23,7 +26,8 @@
 namespace vt {
 
 constexpr int ST_SHORT = 1, ST_NARROW = 2, ST_TOKENS = 4, ST_TREE = 8, ST_FREE_FULL = 16;
-constexpr int TOKENS_ONE_BLOCK = 4096;
+constexpr int ROWS_ONE_BLOCK = 1024, ROWS_CLUSTER = 8;   // rows up to which one block is enough; blocks above
+constexpr int ROWS_CLUSTER_MAX = 16384;
 constexpr int STEP_MAX_REQUESTS = 4096;
 
 struct StepArgs {
@@ -82,16 +86,13 @@ __device__ __forceinline__ void token_row(const StepArgs &A, const int *cu_end, 
     if (A.mask) A.mask[t] = (long long)mask;
 }
 
-__global__ void __launch_bounds__(1024) step_tables_kernel(StepArgs A, int fill_tokens) {
-    extern __shared__ int sm[];
-    int *cu = sm, *need = sm + A.B, *rel = sm + 2 * A.B;   // inclusive prefix sums over the requests
+// The requests' prefix sums and the stack; cu, need and rel are [B] ints of shared memory.
+__device__ __forceinline__ void step_requests(const StepArgs &A, int *cu, int *need, int *rel) {
     __shared__ int wsum[3][32];
     __shared__ int carry[3], flags;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
     if (tid < 3) carry[tid] = 0;
     if (tid == 0) flags = 0;
-    pdl_launch_dependents();
-    pdl_wait();
     const int count = min(max(A.free_count[0], 0), A.free_cap);
     __syncthreads();
     for (int b0 = 0; b0 < A.B; b0 += blockDim.x) {
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(1024) step_tables_kernel(StepArgs A, int fill_
     for (int k = tid; k < given; k += blockDim.x) {
         const int b = first_above(need, A.B, k);
         const int col = clamp_held(A, b) + k - (b ? need[b - 1] : 0);
-        A.table[b * A.table_stride + col] = A.free_blocks[count - 1 - k];
+        if (col < A.width) A.table[b * A.table_stride + col] = A.free_blocks[count - 1 - k];
     }
     __syncthreads();   // the entries taken have been read: the stack may be written
     const int room = A.free_cap - (count - given);
@@ -176,16 +177,52 @@ __global__ void __launch_bounds__(1024) step_tables_kernel(StepArgs A, int fill_
         if (freed > room) f |= ST_FREE_FULL;
         A.status[0] = f;
     }
-    if (!fill_tokens) return;
-    __syncthreads();
-    for (int t = tid; t < A.T; t += blockDim.x) token_row(A, cu, total, A.parents, 0, t);
 }
 
-// The searches and the walks up the parents are chains of dependent reads, so what they read is brought to shared
-// memory first (8300 rows of 256 trees: 7.0 us with them in global memory, both kernels).
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// One block, or a cluster of `blocks` (0: one block, for the requests alone). The searches and the walks up the parents are chains of dependent reads, so what
+// they read is brought to shared memory first.
+__global__ void __launch_bounds__(1024) step_tables_kernel(StepArgs A, int blocks) {
+    extern __shared__ int sm[];   // [3][B] prefix sums, then the parents of 63 + blockDim.x rows
+    int *cu = sm, *par = sm + 3 * A.B;
+    const int tid = threadIdx.x, rank = blocks > 1 ? (int)cluster_rank() : 0;
+    pdl_launch_dependents();
+    pdl_wait();
+    if (rank == 0) step_requests(A, cu, sm + A.B, sm + 2 * A.B);
+    if (blocks == 0) return;   // the rows have a grid of their own
+    if (blocks > 1) {
+        cluster_barrier();   // the first block's tables can be read
+        if (rank > 0)
+            for (int b = tid; b < A.B; b += blockDim.x) cu[b] = A.cu[b + 1];
+    }
+    const int per = (A.T + blocks - 1) / blocks, t1 = min(A.T, (rank + 1) * per);
+    __syncthreads();
+    const int total = cu[A.B - 1];
+    if (!A.parents) {
+#pragma unroll 4
+        for (int t = rank * per + tid; t < t1; t += blockDim.x) token_row(A, cu, total, nullptr, 0, t);
+        return;
+    }
+    for (int t0 = rank * per; t0 < t1; t0 += blockDim.x) {
+        const int p0 = max(t0 - 63, 0), t = t0 + tid;
+        for (int i = p0 + tid; i < min(t0 + (int)blockDim.x, t1); i += blockDim.x) par[i - p0] = A.parents[i];
+        __syncthreads();
+        if (t < t1) token_row(A, cu, total, par, p0, t);
+        __syncthreads();
+    }
+}
+
 constexpr int ROWS_THREADS = 256;
 __global__ void __launch_bounds__(ROWS_THREADS) step_rows_kernel(StepArgs A) {
-    extern __shared__ int sm[];   // [B] ends of the requests, then [63 + ROWS_THREADS] parents
+    extern __shared__ int sm[];   // [B] ends of the requests, then the parents of 63 + ROWS_THREADS rows
     int *par = sm + A.B;
     pdl_launch_dependents();
     pdl_wait();
@@ -231,22 +268,42 @@ extern "C" int vt_step_tables(void *table, long long table_stride, int width, vo
     A.slots = (long long *)slots;
     A.mask = parents ? (long long *)mask : nullptr;
     cudaStream_t s = (cudaStream_t)stream;
-    const bool one = T <= TOKENS_ONE_BLOCK;
+    const int blocks = T <= ROWS_ONE_BLOCK ? 1 : T <= ROWS_CLUSTER_MAX ? ROWS_CLUSTER : 0;
     const int threads = (B <= 256 && T <= 256) ? 256 : 1024;
-    const size_t smem = (size_t)3 * B * sizeof(int);
+    const size_t smem = (size_t)(3 * B + 63 + threads) * sizeof(int);
     if (smem > 40 * 1024) {   // past the default limit together with the static arrays
         const int dev = cur_device();
         static std::atomic<bool> attr[VT_MAX_DEV];
         if (dev < 0 || dev >= VT_MAX_DEV) return VT_EARG;
         if (!attr[dev]) {
             if (cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     3 * STEP_MAX_REQUESTS * (int)sizeof(int)) != cudaSuccess)
+                                     (3 * STEP_MAX_REQUESTS + 63 + 1024) * (int)sizeof(int)) != cudaSuccess)
                 return (int)cudaGetLastError();
             attr[dev] = true;
         }
     }
-    if (int rc = launch_k(step_tables_kernel, dim3(1), dim3(threads), smem, s, true, A, (int)one)) return rc;
-    if (one) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks ? blocks : 1);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (blocks > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = blocks;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (pdl_enabled()) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = n;
+    if (const cudaError_t e = cudaLaunchKernelEx(&cfg, step_tables_kernel, A, blocks)) return (int)e;
+    if (blocks) return (int)cudaGetLastError();
     return launch_k(step_rows_kernel, dim3((T + ROWS_THREADS - 1) / ROWS_THREADS), dim3(ROWS_THREADS),
                     (size_t)(B + 63 + ROWS_THREADS) * sizeof(int), s, true, A);
 }

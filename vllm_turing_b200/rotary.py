@@ -4,8 +4,8 @@ for long contexts; alone (either direction), or in one kernel with the write of 
 Angles come from 64-bit frequencies and are reduced in 64 bits, so far positions keep 32-bit accuracy without a table
 of cosines.
 """
-import ctypes
 import math
+import struct
 from typing import NamedTuple
 
 import torch
@@ -67,7 +67,7 @@ def rope_frequencies(rot_dim, base=10000.0, scaling="none", factor=1.0, original
     return RopeFreqs(turns, scale, rot_dim)
 
 
-_STRIDES8, _STRIDES14 = ctypes.c_longlong * 8, ctypes.c_longlong * 14
+_STRIDES8, _STRIDES14 = struct.Struct("8q").pack, struct.Struct("14q").pack   # int64 arrays for the C entries
 _CODE = {torch.float16: 0, torch.bfloat16: 1}
 
 
@@ -130,7 +130,7 @@ def rotary(q, k, positions, freqs, interleaved=False, transpose=False, q_out=Non
         ks, ko = k.stride(), k_out.stride()
         strides = _STRIDES8(qs[0], qs[1], qo[0], qo[1], ks[0], ks[1], ko[0], ko[1])
     else:
-        strides = _STRIDES8(qs[0], qs[1], qo[0], qo[1])
+        strides = _STRIDES8(qs[0], qs[1], qo[0], qo[1], 0, 0, 0, 0)
     launch("vt_rotary", _build.load().vt_rotary, dev.index, q.data_ptr(), q_out.data_ptr(),
            None if k is None else k.data_ptr(), None if k is None else k_out.data_ptr(), strides,
            positions.data_ptr(), freqs.turns.data_ptr(), freqs.factor, bool(interleaved), bool(transpose), T, Hq, Hkv,

@@ -1,6 +1,6 @@
 """Attention of a step's new tokens over the paged cache (csrc/tree_attn.cu): single tokens, chains, and trees of
 drafted tokens (up to 64 a request) whose mask words come from steptables.step_tables."""
-import ctypes
+import struct
 
 import torch
 
@@ -11,7 +11,7 @@ MAX_NEW = 64
 MAX_GROUP = 128   # query heads to a cached head
 
 
-_STRIDES = ctypes.c_longlong * 10
+_STRIDES = struct.Struct("10q").pack   # an int64 array for the C entry
 _CODE = {torch.float16: 0, torch.bfloat16: 1}
 _ws_words = {}   # (device, D) -> workspace, in 32-bit words
 
