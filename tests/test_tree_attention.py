@@ -136,7 +136,8 @@ def run(c, **kw):
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("trees", [False, True], ids=["chain", "tree"])
 @pytest.mark.parametrize("Hq, Hkv, D", [(6, 1, 256), (24, 4, 256), (8, 2, 128), (4, 4, 64), (7, 1, 80), (10, 2, 192),
-                                        (3, 3, 8), (16, 1, 128), (40, 1, 64), (2, 1, 248)])
+                                        (3, 3, 8), (16, 1, 128), (40, 1, 64), (2, 1, 248), (128, 1, 128),
+                                         (200, 2, 256)])
 def test_heads(Hq, Hkv, D, trees, dtype):
     c = make([1, 5, 64, 129, 300, 17], [1, 5, 3, 8, 4, 0], Hq, Hkv, D, 16, DT[dtype], seed=D + Hq, trees=trees)
     check(c, run(c))
@@ -368,7 +369,8 @@ def test_refusals():
                 dict(k_cache=b(2, 12, 2, 64), v_cache=b(2, 12, 2, 64)), dict(k_cache=wide, v_cache=wide),
                 dict(k_cache=b(0, 16, 2, 64), v_cache=b(0, 16, 2, 64)), dict(max_new=0), dict(max_new=65),
                 dict(cu=i(2)), dict(cu=i(3).long()), dict(seq_lens=i(2).long()), dict(block_table=i(3, 5)),
-                dict(block_table=i(5, 2).t()), dict(mask=i(3)), dict(mask=i(4).long()), dict(out=b(3, 4, 63)), {}):
+                dict(block_table=i(5, 2).t()), dict(block_table=i(2, 0)), dict(mask=i(3)),
+                dict(q=b(3, 258, 64)), dict(mask=i(4).long()), dict(out=b(3, 4, 63)), {}):
         with pytest.raises(ValueError):
             A.tree_attention(**{**good, **bad})
     for bad in (dict(q=b(3, 4, 64).float()), dict(v_cache=b(2, 16, 2, 64).half()), dict(out=b(3, 4, 64).half())):

@@ -255,6 +255,22 @@ template <typename T> __device__ __forceinline__ bool ta_wild(uint32_t half) {
 }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Waits for the phase of `parity` to complete; false when that takes longer than timeout_ns. The bound is each wait's
+// own (a call over a very long context may run longer than it); the timer is read every 1024 polls.
+__device__ __forceinline__ bool ta_wait(uint64_t *bar, uint32_t parity, uint64_t timeout_ns) {
+    uint32_t polls = 0;
+    uint64_t deadline = 0;
+    while (!mbar_try_wait(bar, parity)) {
+        if ((++polls & 1023u) != 0) continue;
+        const uint64_t now = globaltimer();
+        if (deadline == 0) deadline = now + timeout_ns;
+        else if (now > deadline) return false;
+    }
+    return true;
+}
+__device__ __forceinline__ bool ta_warp_wait(uint64_t *bar, uint32_t parity, uint64_t timeout_ns) {
+    return __all_sync(0xffffffffu, ta_wait(bar, parity, timeout_ns)) != 0;
+}
 // K as it lies in the cache, [keys][64 values] rows of 128 bytes: groups of 8 keys `gs` bytes apart (stride offset).
 __device__ __forceinline__ uint64_t ta_k_desc(uint32_t saddr, int gs) {
     uint64_t d = 0;
@@ -444,7 +460,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
     ta_plan<Lay::THREADS>(A, TK, plan, wsum);   // synchronises the block
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t *>(tmem_slot);
-    const uint64_t deadline = globaltimer() + A.timeout_ns;   // of every wait: one that runs out ends them all
+    const uint64_t limit = A.timeout_ns;   // of every wait
 
     if (warp == K_WARP || warp == V_WARP) {
         // ---------------- K and V tiles ----------------
@@ -472,7 +488,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                     mbar_arrive(&segfull[seg % TA_RING]);
                 }
                 __syncwarp();
-            } else if (!warp_wait(&segfull[seg % TA_RING], (uint32_t)(seg / TA_RING) & 1u, deadline)) {
+            } else if (!ta_warp_wait(&segfull[seg % TA_RING], (uint32_t)(seg / TA_RING) & 1u, limit)) {
                 if (lane == 0) report(A.status, ST_PIPE_TIMEOUT | 0x218u);
                 break;
             }
@@ -492,7 +508,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                 if (kt + 1 < kt0 + tiles) ent = entry_of(kt + 1, r0);
                 int ok = 1;
                 if (lane == 0) {
-                    ok = mbar_wait(&empty[s], phase, deadline);
+                    ok = ta_wait(&empty[s], phase, limit);
                     if (!ok) report(A.status, ST_PIPE_TIMEOUT | 0x210u);
                 }
                 if (!__shfl_sync(0xffffffffu, ok, 0)) {
@@ -517,8 +533,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             ++seg;
         }
         if (dead && lane == 0) {   // let the copies already issued land before the shared memory is released
-            const uint64_t d2 = globaltimer() + A.timeout_ns;
-            for (int j = (g > S ? g - S : 0); j < g; ++j) mbar_wait(&full[j % S], (uint32_t)(j / S) & 1u, d2);
+            for (int j = (g > S ? g - S : 0); j < g; ++j) ta_wait(&full[j % S], (uint32_t)(j / S) & 1u, limit);
         }
         __syncwarp();
     } else if (warp == MMA_WARP) {
@@ -532,7 +547,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         int g = 0, seg = 0, ks = 0, vs = 0;   // tiles, segments, ring slots
         uint32_t kphase = 0, vphase = 0;
         auto wait = [&](uint64_t *bar, uint32_t parity, unsigned code) {
-            if (warp_wait(bar, parity, deadline)) {
+            if (ta_warp_wait(bar, parity, limit)) {
                 tc_fence_after();
                 return true;
             }
@@ -578,7 +593,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             ++seg;
         }
         umma_commit_e(drain);   // every MMA issued has completed once it flips
-        warp_wait(drain, 0u, globaltimer() + A.timeout_ns);
+        ta_warp_wait(drain, 0u, limit);
     } else if (warp == Q_WARP) {
         // ---------------- Q of the items ----------------
         // [chunk][row] of 128 bytes (64 values), swizzled: one TMA box a chunk (its tokens past the request's end give
@@ -587,7 +602,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         int round = 0;
         bool ok = true;
         for (int seg = 0; ok; ++seg) {
-            ok = warp_wait(&segfull[seg % TA_RING], (uint32_t)(seg / TA_RING) & 1u, deadline);
+            ok = ta_warp_wait(&segfull[seg % TA_RING], (uint32_t)(seg / TA_RING) & 1u, limit);
             const TaSeg &sg = segs[seg % TA_RING];
             if (!ok || sg.tiles == 0) break;
             const int tok0 = sg.cu0 + sg.rt * A.tile_tokens, h0 = sg.h * A.G;
@@ -595,7 +610,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             for (int c0 = 0; ok && c0 < NCH; c0 += QC, ++round) {
                 const int b = round % QB, nc = min(QC, NCH - c0);
                 uint64_t *bar = QT ? &qbfull[b] : qfull;
-                ok = warp_wait(&qbempty[b], ((uint32_t)(round / QB) & 1u) ^ 1u, deadline);
+                ok = ta_warp_wait(&qbempty[b], ((uint32_t)(round / QB) & 1u) ^ 1u, limit);
                 if (!ok) break;
                 unsigned char *buf = qs + b * Lay::Q_ROUND;
                 if (A.q_map) {
@@ -629,7 +644,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         bool dead = false;
         auto wait = [&](uint64_t *bar, uint32_t parity, unsigned code) {
             if (dead) return;   // the loops go on without data, so that the barriers among these warps stay matched
-            if (!warp_wait(bar, parity, deadline)) {
+            if (!ta_warp_wait(bar, parity, limit)) {
                 if (lane == 0) report(A.status, ST_PIPE_TIMEOUT | code);
                 dead = true;
             }
@@ -1192,7 +1207,7 @@ int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, v
                       void *stream) {
     if (!q || !k_cache || !v_cache || !out || !strides || !block_table || !cu || !seq_lens || B < 1 || T < 0 ||
         max_new < 1 || max_new > TA_MAX_NEW || Hkv < 1 || Hq < Hkv || Hq % Hkv || Hq / Hkv > TA_ROWS || D < 8 || D > 256 ||
-        D % 8 || block_size < 8 || block_size % 8 || table_width < 0 || num_blocks < 1 || num_blocks > 0x7ffffffe ||
+        D % 8 || block_size < 8 || block_size % 8 || table_width < 1 || num_blocks < 1 || num_blocks > 0x7ffffffe ||
         (dtype != 0 && dtype != 1) || !workspace || ((uintptr_t)workspace & 255) ||
         ws_bytes < vt_tree_attention_ws_bytes(max_new, Hq, Hkv, D) || ((uintptr_t)k_cache & 15) ||
         ((uintptr_t)v_cache & 15) || !(scale == scale))

@@ -48,7 +48,7 @@ def _refuse(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask):
     need(B >= 0 and vector(seq_lens, torch.int32, B) and vector(cu, torch.int32, B + 1),
          "tree_attention: seq_lens must be contiguous int32 [B] and cu int32 [B + 1]")
     need(mask is None or vector(mask, torch.int64, T), "tree_attention: mask must be contiguous int64 [T]")
-    raise ValueError("tree_attention: block_table must be int32 [B, width] with contiguous rows")
+    raise ValueError("tree_attention: block_table must be int32 [B, width], width >= 1, with contiguous rows")
 
 
 def tree_attention(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask=None, scale=None, out=None):
@@ -58,7 +58,7 @@ def tree_attention(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask
     A token sees all keys before the step's own and, of those, the ones whose bit is set in its mask word (int64 [T]);
     without a mask, itself and the ones before it. A token that sees nothing gets 0. max_new (1 .. 64): the largest
     number of tokens of a request in this call. Rows of `out` past the last token are left as they were.
-    D % 8 == 0 up to 256, block_size % 8 == 0, Hq a multiple of Hkv (at most 128 times it); scale defaults to D ** -0.5."""
+    The first call on a device must come before any stream capture. D % 8 == 0 up to 256, block_size % 8 == 0, Hq a multiple of Hkv (at most 128 times it); scale defaults to D ** -0.5."""
     qshape, cshape, tshape = q.shape, k_cache.shape, block_table.shape
     max_new = int(max_new)
     if not (len(qshape) == 3 and len(cshape) == 4 and len(tshape) == 2):
@@ -71,7 +71,7 @@ def tree_attention(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask
             and bs >= 8 and bs & 7 == 0 and 1 <= Hkv <= Hq <= MAX_GROUP * Hkv and Hq % Hkv == 0 and _aligned(k_cache, ks)
             and _aligned(v_cache, vs) and 1 <= max_new <= MAX_NEW and vector(seq_lens, torch.int32, B)
             and vector(cu, torch.int32, B + 1) and block_table.dtype == torch.int32
-            and (ts[1] == 1 or tshape[1] <= 1) and (mask is None or vector(mask, torch.int64, T))) and T > 0:
+            and (ts[1] == 1 or tshape[1] == 1) and tshape[1] >= 1 and (mask is None or vector(mask, torch.int64, T))) and T > 0:
         _refuse(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask)
     dt, dev = q.dtype, q.device
     if out is None:
