@@ -293,6 +293,15 @@ def test_lengths_that_do_not_fit():
 
 
 @pytest.mark.gpu
+def test_a_length_far_past_the_table():
+    """The largest length an int holds: every key the table has is context, the step's own tokens are past it."""
+    c = make([80, 40], [4, 2], 6, 2, 128, 16, torch.bfloat16, seed=12)
+    c["lens"][0] = (1 << 31) - 1
+    c["see"][0] = torch.ones(4, 4, dtype=torch.bool)
+    check(c, run(c))
+
+
+@pytest.mark.gpu
 def test_graph_and_streams():
     """Captured once, replayed with other lengths, tables and masks; two captured graphs and two streams at once."""
     c = make([900, 400, 33], [5, 5, 5], 12, 2, 256, 16, torch.bfloat16, seed=7)

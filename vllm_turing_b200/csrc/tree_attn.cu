@@ -119,8 +119,9 @@ __device__ __forceinline__ TaReq ta_request(const TaArgs &A, int b, int tk) {
     TaReq r;
     r.cu0 = A.cu[b];
     r.n = max(A.cu[b + 1] - r.cu0, 0);
-    r.L = max(A.seq_lens[b], 0);
-    r.nt = max(1, (int)(((long long)r.L + tk - 1) / tk));
+    r.L = min(max(A.seq_lens[b], 0), 0x7fff0000);   // the last tile's keys stay within an int
+    // tiles past the table's columns hold nothing to see
+    r.nt = max(1, (int)((min((long long)r.L, (long long)A.width * A.bs) + tk - 1) / tk));
     r.rtn = (min(r.n, A.max_new) + A.tile_tokens - 1) / A.tile_tokens;
     r.units = (long long)A.Hkv * r.rtn * (r.nt + TA_ITEM_COST);
     return r;
