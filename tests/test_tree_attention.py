@@ -440,3 +440,17 @@ def test_context_values_that_are_not_finite():
         assert torch.isfinite(out[:, Hq // 2:]).all() and torch.isfinite(out[:, :Hq // 2, 6]).all()
         c["kc"][page[200 // 16], 200 % 16, 1] = float("nan")
         assert run(c)[:, Hq // 2:].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [400, 1100])
+@pytest.mark.parametrize("Hq, Hkv, D", [(72, 1, 64), (128, 1, 128), (72, 1, 192), (128, 1, 256)])
+def test_segments_of_one_tile(Hq, Hkv, D, B):
+    """More than 64 rows and a few keys a request: a CTA's items are one tile each, so that its row warps go from one
+    segment's "is there another" straight to the next one's."""
+    lens = [1 + (7 * i) % 60 for i in range(B)]
+    c = make(lens, [1] * B, Hq, Hkv, D, 16, torch.bfloat16, seed=D)
+    out = run(c)
+    check(c, out)
+    for _ in range(20):
+        assert torch.equal(run(c), out)

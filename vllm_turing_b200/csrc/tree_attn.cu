@@ -72,7 +72,7 @@ template <int NCH, int REP> struct TaLayout {        // NCH: 64-value chunks of 
     // the 7 that fit, or of 12) + 2, which is how far the K warp can be ahead of the rows
     static constexpr int RING = SLOT >= 32768 ? 8 : 16;
     // barriers and small shared state, bytes (checked in the kernel)
-    static constexpr int BARS = ((2 * MAX_SLOTS + 12 + RING) * 8 + RING * 56 + 40 + GR * 1024 + (6 + RING) * 4 + 127) / 128 * 128;
+    static constexpr int BARS = ((2 * MAX_SLOTS + 12 + RING) * 8 + RING * 56 + 40 + GR * 1024 + (7 + RING) * 4 + 127) / 128 * 128;
     // tensor memory: O | S0 S1 | P0 P1 or Q
     static constexpr int S_COL = DP, Q_COL = S_COL + 2 * TK, P_COL = QT ? S_COL : Q_COL, P_LD = QT ? TK : TK / 2;
     static_assert(Q_COL + (QT ? DP / 2 : TK) <= 512, "tensor memory");
@@ -407,12 +407,12 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
     long long *wsum = reinterpret_cast<long long *>(ml);          // [warps], before
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(hm + (GR == 2 ? 2 : 1));
     uint32_t *wild = tmem_slot + 1;                               // [2 segments][2 words]
-    volatile uint32_t *more = wild + 4;                           // [1] the rows have another segment
-    volatile uint32_t *bad = wild + 5;                            // [TA_RING] 8-row groups not there
+    volatile uint32_t *more = wild + 4;                           // [segment & 1] the rows have another segment
+    volatile uint32_t *bad = wild + 6;                            // [TA_RING] 8-row groups not there
     // what stands between kfull and here, at the most slots, fits the bytes that the host adds to Q and the rings
     static_assert(sizeof(TaSeg) == 56 && sizeof(TaPlan) == 40 &&
                       8 * (2 * MAX_SLOTS + 2 + 2 + 2 + 1 + 2 + 2 + 1 + TA_RING) + TA_RING * (int)sizeof(TaSeg) +
-                              (int)sizeof(TaPlan) + GR * 2 * TA_ROWS * 4 + 4 * (1 + 4 + 1 + TA_RING) <=
+                              (int)sizeof(TaPlan) + GR * 2 * TA_ROWS * 4 + 4 * (1 + 4 + 2 + TA_RING) <=
                           Lay::BARS,
                   "shared state");
     static_assert(Lay::THREADS / 32 * 8 <= GR * 2 * TA_ROWS * 4, "sums of the plan");
@@ -655,9 +655,11 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         // the next segment, if there is one, and its Q into tensor memory
         auto open = [&]() {
             wait(&segfull[seg % TA_RING], (uint32_t)(seg / TA_RING) & 1u, 0x258u);
-            if (threadIdx.x == 0) *more = !dead && segs[seg % TA_RING].tiles != 0;   // one thread decides: the warps'
-            named_sync(TC_EPI_BAR, 128 * GR);                                        // barriers must match
-            if (!*more) return false;
+            // One thread decides, since the warps' barriers must match. Two words in turn: a word is written again only
+            // after the next segment's barrier, which a warp reaches after it has read this one's.
+            if (threadIdx.x == 0) more[seg & 1] = !dead && segs[seg % TA_RING].tiles != 0;
+            named_sync(TC_EPI_BAR, 128 * GR);
+            if (!more[seg & 1]) return false;
             if constexpr (QT) {
                 constexpr int QC = Lay::QC, QB = Lay::QB;
 #pragma unroll
