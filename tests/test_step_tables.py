@@ -247,3 +247,35 @@ def test_refusals():
     n = S.MAX_REQUESTS + 1
     with pytest.raises(ValueError):
         S.step_tables(i(n, 1), i(n), i(4), i(1), i(n), i(n), 16, 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("trees", [False, True])
+def test_lengths_whose_sums_pass_an_int(trees):
+    """cu stops at the largest int (and status says that there are more tokens than rows); the rows that there are
+    belong to the first request."""
+    top, T, bs = (1 << 31) - 1, 40, 16
+    table, held, free, count = [[4, 7, -1], [1, -1, -1], [2, -1, -1]], [2, 1, 1], [9, 8], 2
+    (t, h, f, c), st = on_gpu(table, held, free, count, [5, 10, 3], [top, top, 5], bs, T, [-1] * T if trees else None)
+    assert st.cu.tolist() == [0, top, top, top]
+    assert st.seq_lens.tolist() == [top, top, 8]
+    assert st.status.item() == S.NARROW | S.TOO_MANY | (S.BIG_TREE if trees else 0)
+    assert st.positions.tolist() == [5] * T if trees else st.positions.tolist() == list(range(5, 5 + T))
+    ids = [4, 7]
+    assert st.slots.tolist() == [ids[j // bs] * bs + j % bs if j < 32 else -1 for j in range(5, 5 + T)]
+    assert h.tolist() == held and c.item() == 2 and t.tolist() == table
+
+
+@pytest.mark.gpu
+def test_blocks_whose_sum_passes_an_int():
+    """Requests that need 2^20 blocks each, more than 2^31 in all: the few there are go to none of them."""
+    B, width = 2100, 1 << 20
+    if torch.cuda.mem_get_info()[0] < 20e9:
+        pytest.skip("needs 20 GB")
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")   # noqa: E731
+    table, held, free, count = i(B, width), i(B), i(8) + 3, i(1) + 8
+    held[:5] = width
+    st = S.step_tables(table, held, free, count, i(B) + width, i(B), 1, 0)
+    assert st.status.item() == S.SHORT and count.item() == 8
+    assert held.tolist() == [width] * 5 + [0] * (B - 5) and free.tolist() == [3] * 8
+    assert not table[:5].any() and not (table == 3).any()

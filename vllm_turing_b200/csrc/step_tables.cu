@@ -51,6 +51,12 @@ __device__ __forceinline__ int first_above(const int *incl, int n, int x) {
     return lo;
 }
 
+// a + b for a, b >= 0, at most INT_MAX: the sums are over what the caller's lengths say, and one that wrapped would be
+// searched, and give places in the table, as if it were small. Saturating sums stay sorted in any order of adding.
+__device__ __forceinline__ int sat_add(int a, int b) {
+    return (int)min((unsigned)a + (unsigned)b, (unsigned)INT_MAX);
+}
+
 __device__ __forceinline__ int clamp_held(const StepArgs &A, int b) { return min(max(A.held[b], 0), A.width); }
 
 // One token row: its position, slot and mask word. cu_end[b] = first token after request b; parents of token t at
@@ -93,7 +99,7 @@ __device__ __forceinline__ void step_requests(const StepArgs &A, int *cu, int *n
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
     if (tid < 3) carry[tid] = 0;
     if (tid == 0) flags = 0;
-    const int count = min(max(A.free_count[0], 0), A.free_cap);
+    const int count = min(min(max(A.free_count[0], 0), A.free_cap), INT_MAX - 1);   // below a saturated sum
     __syncthreads();
     for (int b0 = 0; b0 < A.B; b0 += blockDim.x) {
         const int b = b0 + tid;
@@ -116,7 +122,7 @@ __device__ __forceinline__ void step_requests(const StepArgs &A, int *cu, int *n
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int x = __shfl_up_sync(0xffffffffu, v[k], o);
-                if (lane >= o) v[k] += x;
+                if (lane >= o) v[k] = sat_add(v[k], x);
             }
             if (lane == 31) wsum[k][warp] = v[k];
         }
@@ -126,18 +132,19 @@ __device__ __forceinline__ void step_requests(const StepArgs &A, int *cu, int *n
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
+                if (lane >= o) x = sat_add(x, y);
             }
             const int before = carry[warp];
             __syncwarp();
-            wsum[warp][lane] = before + x;
-            if (lane == 31) carry[warp] = before + x;
+            x = sat_add(before, x);
+            wsum[warp][lane] = x;
+            if (lane == 31) carry[warp] = x;
         }
         __syncthreads();
         if (b < A.B) {
-            cu[b] = v[0] + (warp ? wsum[0][warp - 1] : (b0 ? cu[b0 - 1] : 0));
-            need[b] = v[1] + (warp ? wsum[1][warp - 1] : (b0 ? need[b0 - 1] : 0));
-            rel[b] = v[2] + (warp ? wsum[2][warp - 1] : (b0 ? rel[b0 - 1] : 0));
+            cu[b] = sat_add(v[0], warp ? wsum[0][warp - 1] : (b0 ? cu[b0 - 1] : 0));
+            need[b] = sat_add(v[1], warp ? wsum[1][warp - 1] : (b0 ? need[b0 - 1] : 0));
+            rel[b] = sat_add(v[2], warp ? wsum[2][warp - 1] : (b0 ? rel[b0 - 1] : 0));
         }
         __syncthreads();
     }
