@@ -454,3 +454,18 @@ def test_segments_of_one_tile(Hq, Hkv, D, B):
     check(c, out)
     for _ in range(20):
         assert torch.equal(run(c), out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq", [2, 40, 160])
+@pytest.mark.parametrize("masks", [False, True])
+def test_far_more_tokens_than_keys(masks, Hq):
+    """The largest cu an int holds, as step_tables gives it for lengths that add up past one: tokens whose keys would
+    all lie before the first one see nothing; the request after them, past the rows there are, changes nothing."""
+    c = make([300, 90], [3, 2], Hq, 2, 64, 16, torch.bfloat16, seed=13)
+    c["mask"] = torch.full((5,), -1, dtype=torch.int64, device="cuda") if masks else None
+    for n in (300 + 64, 1 << 30, (1 << 31) - 1):
+        c["cu"].copy_(torch.tensor([0, n, n], dtype=torch.int32))
+        assert (run(c)[:3] == 0).all(), n   # max_new is 3
+    c["cu"].copy_(torch.tensor([0, 300 + 60, (1 << 31) - 1], dtype=torch.int32))   # token 60 would see the first key
+    assert (run(c)[:3] == 0).all() != masks   # all bits set: the tokens see four keys

@@ -711,7 +711,8 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         }
         while (has) {
             const TaSeg &sg = segs[seg % TA_RING];
-            const int N = sg.tiles, L = sg.L, ctx = L - sg.n, kt0 = sg.kt0;
+            // (of a request with more tokens than keys, by more than the mask's 64 bits, no token has a key it sees)
+            const int N = sg.tiles, L = sg.L, ctx = max(L - sg.n, -64), kt0 = sg.kt0;
             const int live = min(min(sg.n, A.max_new) - sg.rt * A.tile_tokens, A.tile_tokens) * A.G;
             const int row_i = row / A.G, tok_i = sg.rt * A.tile_tokens + row_i, tok = sg.cu0 + tok_i;
             const bool mine = row < live && tok >= 0 && tok < A.T;
