@@ -469,3 +469,36 @@ def test_far_more_tokens_than_keys(masks, Hq):
         assert (run(c)[:3] == 0).all(), n   # max_new is 3
     c["cu"].copy_(torch.tensor([0, 300 + 60, (1 << 31) - 1], dtype=torch.int32))   # token 60 would see the first key
     assert (run(c)[:3] == 0).all() != masks   # all bits set: the tokens see four keys
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq, D", [(2, 64), (100, 128), (100, 256)])
+def test_segments_longer_than_the_wait_bound(Hq, D):
+    """One request whose share of a CTA takes longer than a wait inside a CTA may: no wait is for a whole segment, so
+    the call is as it was and no status is left."""
+    from vllm_turing_b200 import _build
+    L = _build.load()
+    g = torch.Generator(device="cuda").manual_seed(D)
+    kc, vc = [torch.randn(64, 16, 1, D, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2)]
+    q = torch.randn(1, Hq, D, generator=g, device="cuda").to(torch.bfloat16)
+    width = 1 << 20   # 16M keys, the cache's 64 blocks over and over
+    table = (torch.arange(width, device="cuda", dtype=torch.int32) % 64)[None].contiguous()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")   # noqa: E731
+    args = (q, kc, vc, table, i32([0, 1]), i32([16 * width]), 1)
+    want = A.tree_attention(*args)
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    A.tree_attention(*args)
+    b.record()
+    b.synchronize()
+    assert a.elapsed_time(b) > 0.5   # ms
+    assert L.vt_status(0) == 0
+    try:
+        L.vt_set_wait_bounds(0.2, 0.0)
+        got = A.tree_attention(*args)
+        torch.cuda.synchronize()
+    finally:
+        L.vt_set_wait_bounds(2000.0, 0.0)
+        status = L.vt_status(1)
+    assert status == 0, hex(status)
+    assert torch.equal(got, want)

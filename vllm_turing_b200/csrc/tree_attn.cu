@@ -256,6 +256,11 @@ template <typename T> __device__ __forceinline__ bool ta_wild(uint32_t half) {
 }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// n limits, at most 2^62 ns (added to the timer it must not wrap)
+__device__ __forceinline__ uint64_t ta_times(uint64_t limit, uint64_t n) {
+    constexpr uint64_t MOST = 1ull << 62;
+    return __umul64hi(limit, n) != 0 || limit * n > MOST ? MOST : limit * n;
+}
 // Waits for the phase of `parity` to complete; false when that takes longer than timeout_ns. The bound is each wait's
 // own (a call over a very long context may run longer than it); the timer is read every 1024 polls.
 __device__ __forceinline__ bool ta_wait(uint64_t *bar, uint32_t parity, uint64_t timeout_ns) {
@@ -533,7 +538,12 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             }
             ++seg;
         }
-        if (dead && lane == 0) {   // let the copies already issued land before the shared memory is released
+        if (lane == 0) {
+            if (is_k && dead) {   // no further segment: whoever waits for one need not wait out its limit
+                segs[(seg + 1) % TA_RING].tiles = 0;
+                mbar_arrive(&segfull[(seg + 1) % TA_RING]);
+            }
+            // the copies issued land before the shared memory is released (those that were consumed have)
             for (int j = (g > S ? g - S : 0); j < g; ++j) ta_wait(&full[j % S], (uint32_t)(j / S) & 1u, limit);
         }
         __syncwarp();
@@ -602,10 +612,12 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
         constexpr int QC = Lay::QC, QB = Lay::QB;
         int round = 0;
         bool ok = true;
+        uint64_t tiles = 0;   // of the segment before: the K warp hands out the next one after as many waits of its own
         for (int seg = 0; ok; ++seg) {
-            ok = ta_warp_wait(&segfull[seg % TA_RING], (uint32_t)(seg / TA_RING) & 1u, limit);
+            ok = ta_warp_wait(&segfull[seg % TA_RING], (uint32_t)(seg / TA_RING) & 1u, ta_times(limit, tiles + 1));
             const TaSeg &sg = segs[seg % TA_RING];
             if (!ok || sg.tiles == 0) break;
+            tiles = (uint64_t)sg.tiles;
             const int tok0 = sg.cu0 + sg.rt * A.tile_tokens, h0 = sg.h * A.G;
             const int rows = min(A.tile_tokens, A.max_new) * A.G;
             for (int c0 = 0; ok && c0 < NCH; c0 += QC, ++round) {
@@ -633,7 +645,11 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                 if (lane == 0) mbar_arrive(bar);
             }
         }
-        if (!ok && lane == 0) report(A.status, ST_PIPE_TIMEOUT | 0x2b0u);
+        if (lane == 0) {
+            if (!ok) report(A.status, ST_PIPE_TIMEOUT | 0x2b0u);
+            for (int j = (round > QB ? round - QB : 0); j < round; ++j)   // as the K and V warps do
+                ta_wait(QT ? &qbfull[j % QB] : qfull, (uint32_t)(j / QB) & 1u, limit);
+        }
         __syncwarp();
     } else if (warp < ROW_WARPS) {
         // ---------------- rows: softmax and output ----------------
