@@ -998,7 +998,8 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                 }
                 if (!whole && mine && grp == 0) A.stats[slot * TA_ROWS + row] = make_float2(m, l);
             }
-            if constexpr (REP > 1) {   // the staging area is the Q buffer again
+            if constexpr (REP > 1) {   // the staging area is the Q buffer again, which the next copy writes
+                fence_proxy_async();
                 __syncwarp();
                 if (has && lane == 0) mbar_arrive(&qbempty[0]);
             }
