@@ -152,14 +152,14 @@ int vt_silu_mul_quant(const void *gu, void *q, void *scales, int M, int I, int d
  * the cache, new_lens [B] tokens of this step (negative: the request has ended). In place: block_table rows gain the
  * blocks the step needs, held [B] counts each row's blocks, free_blocks [free_cap] is a stack of free block ids of
  * which the first *free_count are valid (taken from its top in request order; the blocks of ended requests are pushed
- * afterwards). Written: cu [B + 1] first token row of each request, seq_lens [B] = cached + new, positions, slots,
- * mask int64 [T] (rows past the last token: 0, -1, 0), *status = OR of 1 free list too short (a request whose blocks
- * no longer fit, and every one after it, gets none; its tokens without a block have slot -1), 2 a request needs more
- * blocks than the table is wide (it gets none), 4 more tokens than T, 8 a tree of more than 64 tokens (mask 0 past the
- * 64th), 16 free_blocks too small for the blocks given back. parents int32 [T] or NULL: index within its request of
- * each token's parent, -1 for one that follows the context (an index not below the token's own counts as -1); with it
- * positions are cached + depth and mask gets each token's ancestors and itself; without, the tokens form a chain and
- * mask is not written. 1 <= B <= 4096. */
+ * afterwards). Written: cu [B + 1] first token row of each request, seq_lens [B] = cached + new, positions, slots, mask
+ * int64 [T] (rows past the last token: 0, -1, 0), *status = OR of 1 free list too short (a request whose blocks no
+ * longer fit, and every one after it, gets none; its tokens without a block have slot -1, the table entries it wanted
+ * become -1), 2 a request needs more blocks than the table is wide (it gets none, likewise), 4 more tokens than T, 8 a
+ * tree of more than 64 tokens (mask 0 past the 64th), 16 free_blocks too small for the blocks given back. parents int32
+ * [T] or NULL: index within its request of each token's parent, -1 for one that follows the context (an index not below
+ * the token's own counts as -1); with it positions are cached + depth and mask gets each token's ancestors and itself;
+ * without, the tokens form a chain and mask is not written. 1 <= B <= 4096. */
 int vt_step_tables(void *block_table, long long table_stride, int width, void *held, void *free_blocks, int free_cap,
                    void *free_count, const void *cached, const void *new_lens, const void *parents, int B, int T,
                    int block_size, void *cu, void *seq_lens, void *positions, void *slots, void *mask, void *status,
@@ -182,15 +182,15 @@ int vt_rotary_cache(const void *q, void *q_out, const void *k, const void *v, vo
                     int block_size, int dtype, void *stream);
 
 /* Attention of each request's new tokens q [T, Hq, D] over its seq_lens[b] cached keys, the last cu[b + 1] - cu[b] of
- * which are the new tokens themselves: token i sees every key before those and, of the new tokens, those with their
- * bit set in mask[cu[b] + i] (int64 [T]), or tokens 0 .. i with mask NULL. Softmax in 32 bits; a token that sees no
- * key gets 0; keys in blocks whose table entry is outside [0, num_blocks) are not seen, whatever the cache holds
- * where nothing is seen. Hq a multiple of Hkv, at most 128 times it (query head h
- * reads cached head h / (Hq / Hkv)), D a multiple of 8 up to
- * 256, block_size a multiple of 8, caches 16-byte aligned with strides that are multiples of 8 elements, 1 <= max_new
- * <= 64 (tokens of a request past max_new are not computed; rows past cu[B] are left as they were). strides (host, in
- * elements): token and head stride of q and out, then block, row and head stride of k_cache and of v_cache. workspace:
- * vt_tree_attention_ws_bytes bytes, 256-byte aligned, need not be zeroed; calls that may overlap must not share it. */
+ * which are the new tokens themselves: token i sees every key before those and, of the new tokens, those with their bit
+ * set in mask[cu[b] + i] (int64 [T]), or tokens 0 .. i with mask NULL. Softmax in 32 bits; a token that sees no key
+ * gets 0; keys in blocks whose table entry is outside [0, num_blocks) are not seen, whatever the cache holds where
+ * nothing is seen. Hq a multiple of Hkv, at most 128 times it (query head h reads cached head h / (Hq / Hkv)), D a
+ * multiple of 8 up to 256, block_size a multiple of 8, caches 16-byte aligned with strides that are multiples of 8
+ * elements, 1 <= max_new <= 64 (tokens of a request past max_new are not computed; rows past cu[B] are left as they
+ * were). strides (host, in elements): token and head stride of q and out, then block, row and head stride of k_cache
+ * and of v_cache. workspace: vt_tree_attention_ws_bytes bytes, 256-byte aligned, need not be zeroed; calls that may
+ * overlap must not share it. */
 size_t vt_tree_attention_ws_bytes(int max_new, int Hq, int Hkv, int D);
 int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, void *out, const long long *strides,
                       const void *block_table, long long table_stride, int table_width, const void *cu,

@@ -119,3 +119,34 @@ def test_tree_decoding(graph):
         # what o_proj takes: the quantiser's rows are those of the attention's output
         want_q, want_s = scaled_int8_quant_cuda(out.view(T, HQ * D))
         assert torch.equal(quant[0], want_q) and torch.equal(quant[1], want_s)
+
+
+@pytest.mark.gpu
+def test_a_stack_that_runs_out():
+    """Requests that get no blocks, over a table whose entries past what they hold are other requests' blocks: their
+    tokens see what the request holds and nothing of the others."""
+    dev, bs = "cuda", 16
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)   # noqa: E731
+    table = ints([[0, 1, 9, 9], [2, 3, 0, 1], [4, 5, 0, 0], [6, 7, 1, 0], [8, 9, 0, 0]])
+    held, free, count = ints([2] * 5), ints([10, 11]), ints([2])
+    cached, new = [20] * 5, [13, 30, 60, 6, 20]
+    # blocks: 1 more, 2 more (there is one left), 3 more in a row of 4 (too narrow), none, 1 more (after one not served)
+    st = S.step_tables(table, held, free, count, ints(cached), ints(new), bs, sum(new))
+    assert st.status.item() == S.SHORT | S.NARROW
+    assert table.tolist() == [[0, 1, 11, 9], [2, 3, -1, -1], [4, 5, -1, -1], [6, 7, 1, 0], [8, 9, -1, 0]]
+    assert held.tolist() == [3, 2, 2, 2, 2] and count.item() == 1
+    g = torch.Generator(device=dev).manual_seed(3)
+    kc, vc = [torch.randn(12, bs, HKV, D, generator=g, device=dev).to(DT) for _ in range(2)]
+    q = torch.randn(sum(new), HQ, D, generator=g, device=dev).to(DT)
+    out = A.tree_attention(q, kc, vc, table, st.cu, st.seq_lens, max(new))
+    t = 0
+    for b, (c, n) in enumerate(zip(cached, new)):
+        keys, vals = [x[table[b].long().clamp(min=0)].flatten(0, 1) for x in (kc, vc)]
+        places = int(held[b]) * bs
+        for i in range(n):
+            m = min(c + i + 1, places)
+            want, tol = attend(q[t + i], keys[:m], vals[:m])
+            assert ((out[t + i].double() - want).abs() <= tol).all(), (b, i)
+            j = c + i
+            assert st.slots[t + i].item() == (table[b, j // bs].item() * bs + j % bs if j < places else -1)
+        t += n

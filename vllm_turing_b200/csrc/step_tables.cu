@@ -5,8 +5,9 @@
 // needs need[b] = max(0, ceil((cached + new) / bs) - held) more blocks, taken from the top of a stack of free block
 // ids: with P the inclusive prefix sum of need over the requests, request b is served while P[b] <= free_count, and
 // the k-th block given out is free[free_count - 1 - k]. Every quantity is a prefix sum or a search in one, so nothing
-// is sequential in the requests and the result does not depend on timing. new[b] < 0 ends a request: its blocks go
-// back onto the stack, after this step's were taken.
+// is sequential in the requests and the result does not depend on timing. The entries that a request which is not
+// served wanted become -1, no block. new[b] < 0 ends a request: its blocks go back onto the stack, after this step's
+// were taken.
 //
 // Drafted tokens may form a tree: parents[t] is the index (within its request) of token t's parent, -1 for one that
 // follows the context. depth = number of ancestors; position = cached + depth; the mask word has a bit for the token
@@ -160,6 +161,17 @@ __device__ __forceinline__ void step_requests(const StepArgs &A, int *cu, int *n
         const int b = first_above(need, A.B, k);
         const int col = clamp_held(A, b) + k - (b ? need[b - 1] : 0);
         if (col < A.width) A.table[b * A.table_stride + col] = A.free_blocks[count - 1 - k];
+    }
+    // A request that got none keeps its tokens, and seq_lens counts them: its row must not lead to whatever block ids
+    // lie past those it holds.
+    if (served < A.B || (flags & ST_NARROW)) {
+        for (int b = tid >> 5; b < A.B; b += blockDim.x >> 5) {
+            const int n = A.newl[b], h = clamp_held(A, b);
+            const long long want = ((long long)max(A.cached[b], 0) + n + A.bs - 1) / A.bs;
+            if (n < 0 || (b < served && want <= A.width)) continue;
+            const int end = (int)min(want, (long long)A.width);
+            for (int col = h + lane; col < end; col += 32) A.table[b * A.table_stride + col] = -1;
+        }
     }
     __syncthreads();   // the entries taken have been read: the stack may be written
     const int room = A.free_cap - (count - given);

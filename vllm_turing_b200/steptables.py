@@ -18,8 +18,9 @@ from ._launch import launch, refuse_devices, vector
 
 MAX_REQUESTS = 4096
 # bits of StepTables.status
-SHORT = 1        # the free stack ran out: some requests got no new blocks (their tokens without one have slot -1)
-NARROW = 2       # a request needs more blocks than the table has columns (it got none)
+SHORT = 1        # the free stack ran out: some requests got no new blocks (their tokens without one have slot -1, the
+                 # entries of block_table for them are set to -1, which the attention does not look at)
+NARROW = 2       # a request needs more blocks than the table has columns (it got none, likewise)
 TOO_MANY = 4     # more tokens than num_tokens rows
 BIG_TREE = 8     # a tree of more than 64 tokens
 FREE_FULL = 16   # free_blocks too small for the blocks of ended requests
