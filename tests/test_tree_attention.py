@@ -502,3 +502,39 @@ def test_segments_longer_than_the_wait_bound(Hq, D):
         status = L.vt_status(1)
     assert status == 0, hex(status)
     assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_scale", [1.5, 40.0], ids=["", "weights that underflow"])
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("G, n", [(1, 1), (6, 5), (12, 5), (8, 16), (40, 1), (16, 20)])
+@pytest.mark.parametrize("D", [64, 80, 128, 192, 256])
+def test_infinities_of_the_context_stay_infinities(D, G, n, dtype, q_scale):
+    """An infinite value that a row sees with any weight makes the row's value that infinity, one of either sign or a
+    NaN makes it NaN, whatever the number of rows and wherever the context is cut; the rest does not change."""
+    inf, nan = float("inf"), float("nan")
+    c = make([n + 1, 300 + n, 20000], [n, n, n], 2 * G, 2, D, 16, DT[dtype], seed=D + G, q_scale=q_scale, trees=n > 1)
+    clean = run(c)
+    check(c, clean)
+    puts = {0: [(0, 0, 0, inf), (0, 1, D - 1, -inf)],
+            1: [(299, 0, 3, -inf), (150, 0, 3, -inf), (5, 0, 7, inf), (290, 0, 7, -inf), (130, 1, 9, nan), (299, 1, 60, inf)],
+            2: [(0, 0, 0, inf), (9999, 0, 1, -inf), (19999 - n, 0, 2, inf), (3, 0, 4, inf), (19000, 0, 4, -inf),
+                (12345, 0, 5, nan), (7777, 1, D - 1, inf)] + [(j, 1, 8, inf) for j in range(0, 19000, 500)]}
+    want = clean.clone()
+    for b, where in puts.items():
+        rows = slice(c["host_cu"][b], c["host_cu"][b + 1])
+        seen = {}
+        for j, h, col, x in where:
+            c["vc"][c["table"][b, j // 16].long(), j % 16, h, col] = x
+            seen[h, col] = seen.get((h, col), 0.0) + x
+        for (h, col), x in seen.items():
+            want[rows, h * G:(h + 1) * G, col] = x
+    out = run(c)
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out.nan_to_num(7.0, inf, -inf), want.nan_to_num(7.0, inf, -inf))
+    # a NaN in a query: its row alone
+    c["q"][n, 0, 0] = nan
+    out = run(c)
+    assert out[n, 0].isnan().all()
+    want[n, 0] = nan
+    assert torch.equal(out.nan_to_num(7.0, inf, -inf), want.nan_to_num(7.0, inf, -inf))

@@ -39,7 +39,10 @@
 //
 // What nothing sees must not matter, whatever the memory holds: scores are selected, not added to; in the tiles that
 // reach past ctx the rows of V past L are set to zero in shared memory, and infinities and NaN in the step's own rows
-// are taken out there (0 x inf is NaN) and added to the rows that see them at the end.
+// are taken out there (0 x inf is NaN) and added to the rows that see them at the end. Those of the context stay: every
+// row sees them. But a weight may be 0 in the products where it is not by definition (a replica's for the keys of the
+// others, one that underflows), so a sum that came out as NaN has its column of the context looked through, and takes
+// the sum of the infinities and NaN found there (ta_context_wild). That costs nothing where sums are finite.
 #include <math.h>
 
 #include "tc_core.cuh"
@@ -376,6 +379,40 @@ __device__ __forceinline__ uint32_t ta_seen(unsigned long long see, int kk0, int
     if (jj < 0) return (uint32_t)(see << -jj) | ((1u << -jj) - 1u);
     return jj < 64 ? (uint32_t)(see >> jj) : 0u;
 }
+
+// Bit e of x and of y: some value of column c + e, of the keys j0 .. j1 - 1 of request b and cached head h, is +inf and
+// is -inf; a NaN counts as both. Called by whole warps on uniform values; the lanes share out the keys.
+template <typename T, int NV>
+__device__ __noinline__ uint2 ta_context_wild(const TaArgs &A, int b, int h, int j0, int j1, int c) {
+    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;   // exponent; the mantissa is below it
+    const int *trow = A.table + (long long)b * A.table_stride;
+    uint32_t pos = 0, neg = 0;
+    for (int j = j0 + (int)(threadIdx.x & 31); j < j1; j += 32) {
+        const int page = j / A.bs;
+        if (page >= A.width) break;
+        const int blk = trow[page];
+        if (blk < 0 || blk >= A.num_blocks) continue;
+        const T *v = reinterpret_cast<const T *>(A.v) + blk * A.v_b + (j - page * A.bs) * A.v_r + h * A.v_h + c;
+#pragma unroll
+        for (int i = 0; i < NV / 8; ++i) {
+            if (c + 8 * i >= A.D) break;
+            const uint4 x = *reinterpret_cast<const uint4 *>(v + 8 * i);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t u = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+                if ((u & E) != E) continue;
+                const bool nan = (u & (E ^ 0x7fffu)) != 0;
+                if (nan || !(u & 0x8000u)) pos |= 1u << (8 * i + e);
+                if (nan || (u & 0x8000u)) neg |= 1u << (8 * i + e);
+            }
+        }
+    }
+    return make_uint2(__reduce_or_sync(0xffffffffu, pos), __reduce_or_sync(0xffffffffu, neg));
+}
+
+// x f for a weight f that is 0 only by underflow: an infinity stays one
+__device__ __forceinline__ float ta_scaled(float x, float f) { return isfinite(x) ? x * f : x; }
 
 // ---- the kernel ------------------------------------------------------------------------------------------------------
 template <typename T, int NCH, int REP>
@@ -893,9 +930,22 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             const size_t slot = (size_t)(2 * blockIdx.x + (sg.head ? 0 : 1));
             T *dst = reinterpret_cast<T *>(A.out) + (long long)tok * A.o_t +
                      (long long)(sg.h * A.G + row - row_i * A.G) * A.o_h;
-            // NV values of the row from column c: the parts go to the workspace in 32 bits, a whole item's to the output
-            auto put = [&](auto &o, int c) {
+            // NV values of the row from column c: the parts go to the workspace in 32 bits, a whole item's to the output.
+            // All lanes of the warp call it; `ok` is false where the row is none.
+            auto put = [&](auto &o, int c, bool ok) {
                 constexpr int NV = sizeof(o) / sizeof(float);
+                bool nan = false;
+#pragma unroll
+                for (int e = 0; e < NV; ++e) nan |= o[e] != o[e];
+                if (__any_sync(0xffffffffu, ok && nan && l == l)) {   // (scores that are NaN make l, and the row, NaN)
+                    const uint2 f = ta_context_wild<T, NV>(A, sg.b, sg.h, kt0 * TK, min(ctx, (kt0 + N) * TK), c);
+#pragma unroll
+                    for (int e = 0; e < NV; ++e) {
+                        const bool p = (f.x >> e) & 1u, n = (f.y >> e) & 1u;
+                        if (p || n) o[e] = p && n ? NAN : p ? INFINITY : -INFINITY;
+                    }
+                }
+                if (!ok) return;
                 if (wn) {   // the values taken out above, for the rows that see them
                     for (unsigned long long left = wn; left; left &= left - 1) {
                         const int j = ctx + __ffsll((long long)left) - 1, page = j / A.bs;
@@ -970,10 +1020,11 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                         }
                     }
                     named_sync(TC_EPI_BAR, 128);
-                    if (mine && !dead) {
+                    const bool ok = mine && !dead;
 #pragma unroll 2
-                        for (int c = part * (width / REP); c < (part + 1) * (width / REP); c += 8) {
-                            float r[8] = {};
+                    for (int c = part * (width / REP); c < (part + 1) * (width / REP); c += 8) {
+                        float r[8] = {};
+                        if (ok) {
 #pragma unroll
                             for (int k = 0; k < REP; ++k) {
                                 const float4 *y = reinterpret_cast<const float4 *>(area + (k * RR + row) * ld + c);
@@ -981,8 +1032,8 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                                 r[0] += a.x, r[1] += a.y, r[2] += a.z, r[3] += a.w;
                                 r[4] += b.x, r[5] += b.y, r[6] += b.z, r[7] += b.w;
                             }
-                            put(r, c0 + c);
                         }
+                        put(r, c0 + c, ok);
                     }
                     if (has) named_sync(TC_EPI_BAR, 128);
                 }
@@ -994,7 +1045,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                     float o[32];
                     tmem_ld32(lane_base + (uint32_t)c, *reinterpret_cast<uint32_t(*)[32]>(o));
                     tmem_ld_wait();
-                    if (mine && !dead) put(o, c);
+                    put(o, c, mine && !dead);
                 }
                 if (!whole && mine && grp == 0) A.stats[slot * TA_ROWS + row] = make_float2(m, l);
             }
@@ -1075,10 +1126,8 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
                         m = mn;
                         l = l * f + w * st.y;
 #pragma unroll
-                        for (int e = 0; e < TJ_COLS; ++e) {   // a part without keys may hold anything
-                            const float o = f != 0.0f ? acc[e] * f : 0.0f;
-                            acc[e] = w != 0.0f ? __fmaf_rn(w, v[e], o) : o;
-                        }
+                        for (int e = 0; e < TJ_COLS; ++e)   // (a part that is all hidden from the row holds zeros)
+                            acc[e] = __fmaf_rn(isfinite(v[e]) ? w : 1.0f, v[e], ta_scaled(acc[e], f));
                     }
                 }
             }
@@ -1095,7 +1144,7 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
                         m = mn;
                         l = l * f + g * st.y;
 #pragma unroll
-                        for (int e = 0; e < TJ_COLS; ++e) acc[e] = acc[e] * f + g * acc_sm[w][e][lane];
+                        for (int e = 0; e < TJ_COLS; ++e) acc[e] = ta_scaled(acc[e], f) + ta_scaled(acc_sm[w][e][lane], g);
                     }
                 }
                 __syncthreads();
