@@ -279,3 +279,16 @@ def test_blocks_whose_sum_passes_an_int():
     assert st.status.item() == S.SHORT and count.item() == 8
     assert held.tolist() == [width] * 5 + [0] * (B - 5) and free.tolist() == [3] * 8
     assert not table[:5].any() and not (table == 3).any()
+
+
+@pytest.mark.gpu
+def test_an_empty_stack():
+    """free_blocks without an entry: what needs a block is short of it, what is given back has no room."""
+    i = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")   # noqa: E731
+    for cached, new, status, slots in (([3, 5], [2, 3], 0, [3, 4, 13, 14, 15, -1]),
+                                       ([3, 7], [2, 3], S.SHORT, [3, 4, 15, -1, -1, -1]),
+                                       ([3, 5], [-1, 3], S.FREE_FULL, [13, 14, 15, -1, -1, -1])):
+        table, held, free, count = i([[0, -1], [1, -1]]), i([1, 1]), i([]), i([0])
+        st = S.step_tables(table, held, free, count, i(cached), i(new), 8, 6)
+        assert st.status.item() == status and st.slots.tolist() == slots and count.item() == 0
+        assert held.tolist() == [0 if new[0] < 0 else 1, 1]

@@ -262,8 +262,9 @@ extern "C" int vt_step_tables(void *table, long long table_stride, int width, vo
                               int free_cap, void *free_count, const void *cached, const void *new_lens,
                               const void *parents, int B, int T, int block_size, void *cu, void *seq_lens,
                               void *positions, void *slots, void *mask, void *status, void *stream) {
-    if (!table || !held || !free_blocks || !free_count || !cached || !new_lens || !cu || !seq_lens || !status ||
-        B < 1 || B > STEP_MAX_REQUESTS || T < 0 || width < 1 || table_stride < width || free_cap < 0 ||
+    // (an empty stack has no address)
+    if (!table || !held || (free_cap > 0 && !free_blocks) || !free_count || !cached || !new_lens || !cu || !seq_lens ||
+        !status || B < 1 || B > STEP_MAX_REQUESTS || T < 0 || width < 1 || table_stride < width || free_cap < 0 ||
         block_size < 1 || (T > 0 && (!positions || !slots)) || (parents && T > 0 && !mask))
         return VT_EARG;
     StepArgs A{};
