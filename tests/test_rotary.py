@@ -269,3 +269,14 @@ def test_refusals():
                 dict(rot_dim=32, scaling="llama3", factor=2.0, original_length=10, low_freq_factor=4.0)):
         with pytest.raises(ValueError):
             R.rope_frequencies(device="cpu", **bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [128, 36])
+def test_a_cache_without_blocks(D):
+    """No slot is inside it: q is rotated, nothing is written."""
+    q, k, pos = heads(5, 4, D, torch.bfloat16, 1), heads(5, 2, D, torch.bfloat16, 2), torch.arange(5, device="cuda")
+    f = R.rope_frequencies(12)
+    kc = torch.empty(0, 16, 2, D, dtype=torch.bfloat16, device="cuda")
+    out = R.rotary_cache(q, k, k, pos, pos, kc, torch.empty_like(kc), f)
+    assert torch.equal(out, R.rotary(q, None, pos, f)[0])

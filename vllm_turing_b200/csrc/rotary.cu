@@ -419,8 +419,10 @@ int vt_rotary_cache(const void *q, void *q_out, const void *k, const void *v, vo
     A.rot = rot;
     A.bs = block_size;
     A.q_rest = q != q_out;
-    if (!rot_args_ok(A) || Hkv < 1 || (Hq && (!q || !q_out)) || !k || !v || !k_cache || !v_cache || !slots ||
-        num_blocks < 0 || block_size < 1 || (dtype != 0 && dtype != 1))
+    // (a cache without blocks has no address)
+    if (!rot_args_ok(A) || Hkv < 1 || (Hq && (!q || !q_out)) || !k || !v ||
+        (num_blocks > 0 && (!k_cache || !v_cache)) || !slots || num_blocks < 0 || block_size < 1 ||
+        (dtype != 0 && dtype != 1))
         return VT_EARG;
     A.num_slots = num_blocks * block_size;
     if (T == 0) return 0;
