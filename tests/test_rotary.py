@@ -280,3 +280,38 @@ def test_a_cache_without_blocks(D):
     kc = torch.empty(0, 16, 2, D, dtype=torch.bfloat16, device="cuda")
     out = R.rotary_cache(q, k, k, pos, pos, kc, torch.empty_like(kc), f)
     assert torch.equal(out, R.rotary(q, None, pos, f)[0])
+
+
+def test_inputs_that_require_a_gradient():
+    """No call records one, so none takes an input that asks for it (under no_grad the next refusal is the device)."""
+    f = R.rope_frequencies(32, device="cpu")
+    b = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)   # noqa: E731
+    pos = torch.zeros(3, dtype=torch.int64)
+    q, k, c = b(3, 4, 64), b(3, 2, 64), b(2, 8, 2, 64)
+    for wanting in ((q,), (k,), (q, k)):
+        for x in wanting:
+            x.requires_grad_()
+        for args in ((q, k, pos, f), (q, q, pos, f)) if q.requires_grad else ((q, k, pos, f),):
+            with pytest.raises(ValueError, match="gradient"):
+                R.rotary(*args)
+        for args in ((q, k, b(3, 2, 64)), (b(3, 4, 64), b(3, 2, 64), k)) if k.requires_grad else ((q, k, k),):
+            with pytest.raises(ValueError, match="gradient"):
+                R.rotary_cache(*args, pos, pos, c, c, f)
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+            R.rotary(q, k, pos, f)
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+            R.rotary_cache(q, k, k, pos, pos, c, c, f)
+        for x in wanting:
+            x.requires_grad_(False)
+
+
+@pytest.mark.gpu
+def test_the_custom_ops_refuse_a_gradient_too():
+    f = R.rope_frequencies(32)
+    q, k, pos = heads(5, 4, 64, torch.bfloat16, 1), heads(5, 2, 64, torch.bfloat16, 2), torch.arange(5, device="cuda")
+    q.requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        torch.ops.vllm_turing.rotary_(torch.empty_like(k), None, k, q, pos, f.turns, f.factor, True, False)
+    with torch.no_grad():
+        out, _ = R.rotary(q, k, pos, f)
+    assert torch.equal(out, R.rotary(q.detach(), None, pos, f)[0])

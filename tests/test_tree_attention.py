@@ -538,3 +538,15 @@ def test_infinities_of_the_context_stay_infinities(D, G, n, dtype, q_scale):
     assert out[n, 0].isnan().all()
     want[n, 0] = nan
     assert torch.equal(out.nan_to_num(7.0, inf, -inf), want.nan_to_num(7.0, inf, -inf))
+
+
+def test_inputs_that_require_a_gradient():
+    b = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)   # noqa: E731
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)   # noqa: E731
+    for which in range(3):
+        x = [b(3, 4, 64), b(2, 16, 2, 64), b(2, 16, 2, 64)]
+        x[which].requires_grad_()
+        with pytest.raises(ValueError, match="gradient"):
+            A.tree_attention(*x, i(2, 5), i(3), i(2), 5)
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+            A.tree_attention(*x, i(2, 5), i(3), i(2), 5)

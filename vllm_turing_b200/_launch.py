@@ -34,6 +34,14 @@ def refuse_dtypes(what, *tensors):
     raise TypeError(f"{what}: one dtype, float16 or bfloat16, got {[str(t.dtype) for t in tensors if t is not None]}")
 
 
+def refuse_grad(what, hint=""):
+    raise ValueError(f"{what}: an input requires a gradient, which this call does not record: call it under "
+                     f"torch.no_grad(), or detach the input{hint}")
+
+
+grad_enabled = torch.is_grad_enabled
+
+
 def vector(t, dtype, n):
     """A contiguous 1-D tensor of n elements."""
     return t.dtype == dtype and t.shape == (n,) and t.is_contiguous()

@@ -11,7 +11,7 @@ from typing import NamedTuple
 import torch
 
 from . import _build
-from ._launch import launch, need, refuse_devices, refuse_dtypes, vector
+from ._launch import grad_enabled, launch, need, refuse_devices, refuse_dtypes, refuse_grad, vector
 
 SCALINGS = ("none", "linear", "ntk", "yarn", "llama3")
 MAX_ROT = 1024
@@ -92,8 +92,11 @@ def rotary(q, k, positions, freqs, interleaved=False, transpose=False, q_out=Non
     """(q_out, k_out): q [T, Hq, D] and k [T, Hkv, D] (or None) with the first freqs.rot_dim values of each head
     rotated by positions (int64 [T]); the rest copied. Any token and head strides. q_out / k_out are new tensors unless
     given; they may be q and k themselves. transpose applies the transposed map: the gradient with respect to the input,
-    given the gradient of the output (and, for factor 1, the rotation back)."""
+    given the gradient of the output (and, for factor 1, the rotation back). The call itself is not recorded for
+    autograd, and refuses inputs that ask for it."""
     need(q is not None and q.dim() == 3, "rotary: q must be [T, heads, D]")
+    if grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        refuse_grad("rotary", " (transpose=True is the gradient's map)")
     qshape = q.shape
     T, Hq, D = qshape
     if q_out is None:
@@ -143,6 +146,8 @@ def rotary_cache(q, k, v, positions, slots, k_cache, v_cache, freqs, interleaved
     of the paged cache k_cache, v_cache [num_blocks, block_size, Hkv, D] (any strides, last dimension contiguous). A
     token whose slot is outside the cache (step_tables gives -1) writes no k and v. Slots inside it must differ."""
     need(q is not None and q.dim() == 3 and k.dim() == 3, "rotary_cache: q and k must be [T, heads, D]")
+    if grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        refuse_grad("rotary_cache")
     qshape = q.shape
     T, Hq, D = qshape
     Hkv = k.shape[1]

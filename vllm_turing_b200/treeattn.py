@@ -5,7 +5,7 @@ import struct
 import torch
 
 from . import _build
-from ._launch import launch, need, refuse_devices, refuse_dtypes, vector
+from ._launch import grad_enabled, launch, need, refuse_devices, refuse_dtypes, refuse_grad, vector
 
 MAX_NEW = 64
 MAX_GROUP = 128   # query heads to a cached head
@@ -58,11 +58,15 @@ def tree_attention(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask
     A token sees all keys before the step's own and, of those, the ones whose bit is set in its mask word (int64 [T]);
     without a mask, itself and the ones before it. A token that sees nothing gets 0. max_new (1 .. 64): the largest
     number of tokens of a request in this call. Rows of `out` past the last token are left as they were.
-    The first call on a device must come before any stream capture. D % 8 == 0 up to 256, block_size % 8 == 0, Hq a multiple of Hkv (at most 128 times it); scale defaults to D ** -0.5."""
+    The first call on a device must come before any stream capture. D % 8 == 0 up to 256, block_size % 8 == 0, Hq a
+    multiple of Hkv (at most 128 times it); scale defaults to D ** -0.5. Not recorded for autograd: inputs that require a
+    gradient are refused."""
     qshape, cshape, tshape = q.shape, k_cache.shape, block_table.shape
     max_new = int(max_new)
     if not (len(qshape) == 3 and len(cshape) == 4 and len(tshape) == 2):
         _refuse(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask)
+    if grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        refuse_grad("tree_attention")
     T, Hq, D = qshape
     nb, bs, Hkv, _ = cshape
     B = tshape[0]
