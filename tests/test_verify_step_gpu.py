@@ -150,3 +150,28 @@ def test_a_stack_that_runs_out():
             j = c + i
             assert st.slots[t + i].item() == (table[b, j // bs].item() * bs + j % bs if j < places else -1)
         t += n
+
+
+@pytest.mark.parametrize("layout", ["blocks", "heads", "joint"])
+def test_moving_an_accepted_path(layout):
+    """The lines that INTEGRATION.md gives for it, over every layout of a cache that the operators take."""
+    import os
+    import textwrap
+    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")) as f:
+        lines = textwrap.dedent([b for b in f.read().split("```python\n") if "slots[path]" in b][0].split("```")[0]
+                                .replace("\n  ", "\n").lstrip())
+    nb, block_size, H, d = 5, 4, 2, 3
+    if layout == "heads":
+        k_cache, v_cache = [torch.randn(nb, H, block_size, d).transpose(1, 2) for _ in range(2)]
+    elif layout == "joint":
+        both = torch.randn(nb, 2, block_size, H, d)
+        k_cache, v_cache = both[:, 0], both[:, 1]
+    else:
+        k_cache, v_cache = [torch.randn(nb, block_size, H, d) for _ in range(2)]
+    k0, v0 = k_cache.clone(), v_cache.clone()
+    slots, path = torch.tensor([18, 19, 4, 5, 6, 7, 12]), torch.tensor([0, 2, 3, 6])
+    exec(lines, dict(slots=slots, path=path, k_cache=k_cache, v_cache=v_cache, block_size=block_size))
+    for c, c0 in ((k_cache, k0), (v_cache, v0)):
+        want = c0.reshape(-1, H, d).clone()
+        want[slots[:4]] = c0.reshape(-1, H, d)[slots[path]]
+        assert torch.equal(c.reshape(-1, H, d), want)
