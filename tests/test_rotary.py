@@ -315,3 +315,48 @@ def test_the_custom_ops_refuse_a_gradient_too():
     with torch.no_grad():
         out, _ = R.rotary(q, k, pos, f)
     assert torch.equal(out, R.rotary(q.detach(), None, pos, f)[0])
+
+
+MANY = [  # T, Hq, Hkv, D, rot, block: several shares of heads a warp, one after the other, over most of the GPU's warps
+    (8193, 24, 4, 256, 64, 16), (4099, 32, 8, 128, 128, 16), (9001, 5, 1, 80, 80, 24), (6007, 20, 2, 96, 32, 8),
+    (20011, 3, 1, 64, 16, 32), (5003, 64, 8, 192, 96, 64), (70001, 1, 1, 8, 0, 8), (3001, 40, 3, 256, 256, 16),
+    (2500, 9, 2, 80, 20, 16), (2203, 4, 2, 96, 24, 16),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("inter", [False, True], ids=["half", "interleaved"])
+@pytest.mark.parametrize("shape", MANY, ids=str)
+def test_prompts(shape, inter, dtype):
+    """Prompt-sized calls, every row: alone in both directions and in place, and with the cache write, where some tokens
+    have no place; q, k and v as columns of one wider result."""
+    T, Hq, Hkv, D, rot, bs = shape
+    dt = DT[dtype]
+    g = torch.Generator(device="cuda").manual_seed(T)
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, generator=g, device="cuda").to(dt)
+    q, k, v = [x.view(T, -1, D) for x in qkv.split((Hq * D, Hkv * D, Hkv * D), dim=1)]
+    pos = torch.randint(0, 200000, (T,), generator=g, device="cuda")
+    f = R.rope_frequencies(rot, 500000.0, "yarn", 4.0, 32768)
+    w = f.turns.cpu() * 2 * math.pi
+    for transpose in (False, True):
+        yq, yk = R.rotary(q, k, pos, f, inter, transpose)
+        near(yq, *rotated(q, pos, w, f.factor, rot, inter, transpose))
+        near(yk, *rotated(k, pos, w, f.factor, rot, inter, transpose))
+        both = qkv.clone()
+        qi, ki, vi = [x.view(T, -1, D) for x in both.split((Hq * D, Hkv * D, Hkv * D), dim=1)]
+        R.rotary(qi, ki, pos, f, inter, transpose, qi, ki)
+        assert torch.equal(qi, yq) and torch.equal(ki, yk) and torch.equal(vi, v)
+    yq, yk = R.rotary(q, k, pos, f, inter)
+    nb = -(-T // bs) + 1
+    slots = torch.randperm(nb * bs, generator=g, device="cuda")[:T]
+    slots[torch.rand(T, generator=g, device="cuda") < 0.1] = -1
+    slots[T // 3] = nb * bs
+    kept = (slots >= 0) & (slots < nb * bs)
+    for layout in LAYOUTS:
+        kc, vc = make_cache(layout, nb, bs, Hkv, D, dt)
+        want_k, want_v = kc.clone(), vc.clone()
+        at = slots[kept]
+        want_k[at // bs, at % bs], want_v[at // bs, at % bs] = yk[kept], v[kept]
+        out = R.rotary_cache(q, k, v, pos, slots, kc, vc, f, inter)
+        assert torch.equal(out, yq) and torch.equal(kc, want_k) and torch.equal(vc, want_v)

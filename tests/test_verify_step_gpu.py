@@ -175,3 +175,56 @@ def test_moving_an_accepted_path(layout):
         want = c0.reshape(-1, H, d).clone()
         want[slots[:4]] = c0.reshape(-1, H, d)[slots[path]]
         assert torch.equal(c.reshape(-1, H, d), want)
+
+
+@pytest.mark.gpu
+def test_the_custom_ops_in_a_traced_step():
+    """The four custom ops as a traced graph holds them: traced with fake tensors, run, and compared with the calls."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    dev, ops = "cuda", torch.ops.vllm_turing
+    g = torch.Generator(device=dev).manual_seed(9)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)   # noqa: E731
+    f = R.rope_frequencies(ROT, 10000.0, device=dev)
+    new, most = [3, 5, 1], 5
+    T = sum(new) + 2
+    parents = ints([-1, 0, 0, -1, 0, 1, 1, 0, -1, -1, -1])
+    q, k, v = [torch.randn(T, h, D, generator=g, device=dev).to(DT) for h in (HQ, HKV, HKV)]
+
+    def state():
+        st = S.alloc_tables(3, T, True, torch.device(dev))
+        caches = [torch.zeros(12, BS, HKV, D, dtype=DT, device=dev) for _ in range(2)]
+        return [torch.full((3, 4), -1, dtype=torch.int32, device=dev), ints([0] * 3),
+                torch.arange(12, dtype=torch.int32, device=dev), ints([12]), *st, *caches]
+
+    def step(table, held, free, count, cu, seq_lens, positions, slots, mask, status, kc, vc):
+        cached = torch.zeros_like(held)
+        ops.step_tables_(table, held, free, count, cached, lens, BS, parents, cu, seq_lens, positions, slots, mask, status)
+        qr, qk, kr = torch.empty_like(q), torch.empty_like(q), torch.empty_like(k)
+        ops.rotary_cache_(qr, q, k, v, positions, slots, kc, vc, f.turns, f.factor, False)
+        ops.rotary_(qk, kr, q, k, positions, f.turns, f.factor, False, False)
+        out = torch.zeros_like(q)
+        ops.tree_attention_(out, qr, kc, vc, table, cu, seq_lens, most, mask, None)
+        return out, qr, qk, kr
+
+    lens = ints(new)
+    graph = make_fx(step, tracing_mode="fake", _allow_non_fake_inputs=True)(*state())
+    names = str([n.target for n in graph.graph.nodes if n.op == "call_function"])
+    for op in ("step_tables_", "rotary_cache_", "rotary_", "tree_attention_"):
+        assert f"vllm_turing.{op}" in names
+    traced, direct = state(), state()
+    got = graph(*traced)
+    table, held, free, count, *tables, kc, vc = direct
+    st = S.step_tables(table, held, free, count, ints([0] * 3), lens, BS, T, parents, S.StepTables(*tables))
+    qr = R.rotary_cache(q, k, v, st.positions, st.slots, kc, vc, f)
+    qk, kr = R.rotary(q, k, st.positions, f)
+    out = A.tree_attention(qr, kc, vc, table, st.cu, st.seq_lens, most, mask=st.mask, out=torch.zeros_like(q))
+    for a, b in zip((*got, *traced), (out, qr, qk, kr, *direct)):
+        assert torch.equal(a, b)
+    assert st.status.item() == 0 and out[:sum(new)].any() and not out[sum(new):].any()
+    # without parents: no mask
+    chain = state()
+    ops.step_tables_(*chain[:4], ints([0] * 3), lens, BS, None, *chain[4:8], None, chain[9])
+    want = S.step_tables(*state()[:4], ints([0] * 3), lens, BS, T)
+    assert want.mask is None
+    for a, b in zip(chain[4:8] + [chain[9]], (want.cu, want.seq_lens, want.positions, want.slots, want.status)):
+        assert torch.equal(a, b)
