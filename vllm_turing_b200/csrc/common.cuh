@@ -188,9 +188,14 @@ template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t u) {
     const T *h = reinterpret_cast<const T *>(&u);
     return make_float2(t2f<T>(h[0]), t2f<T>(h[1]));
 }
-template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-    T h[2] = {f2t<T>(a), f2t<T>(b)};
-    return *reinterpret_cast<uint32_t *>(h);
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
 }
 template <typename T> __device__ __forceinline__ float rnd(float x) { return t2f<T>(f2t<T>(x)); }
 

@@ -14,9 +14,8 @@
 // memory asynchronously, makes the token's sines and cosines (a chain of loads and arithmetic of about 2 us) and writes
 // the share that has arrived: first the vectors that pass through, then the rotated ones, a pair of vectors a lane over
 // all heads of the share, so that no lane idles where only part of the head rotates. Warps do not wait for one another.
-// Everything else, larger heads
-// or sizes and addresses that vectors do not fit, takes the second kernel, a unit (vector or element, and its partner)
-// a thread.
+// Everything else, larger heads or sizes and addresses that vectors do not fit, takes the second kernel, a unit (vector
+// or element, and its partner) a thread.
 #include "common.cuh"
 #include "host_util.h"
 
@@ -151,15 +150,6 @@ __device__ __forceinline__ void ro_copy16(void *dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
-template <typename T> __device__ __forceinline__ uint32_t ro_pack(float a, float b);
-template <> __device__ __forceinline__ uint32_t ro_pack<__half>(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <> __device__ __forceinline__ uint32_t ro_pack<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
 
 // Shared memory of a block: two shares a warp, [warp][2][RO_ROWS][32 lanes] vectors, then the cosines [warp][128].
 constexpr int RO_SMEM = RO_THREADS / 32 * (2 * RO_ROWS * 32 * 16 + 128 * 8);
@@ -194,7 +184,8 @@ __global__ void __launch_bounds__(RO_THREADS, RO_BLOCKS) rotary_warp_kernel(cons
             for (int i = 0; i < RO_ROWS; ++i) {
                 const int e = sh * hpw + sub + i * step;
                 if (e >= E) break;
-                ro_copy16(&buf[b][i][lane], e < A.Hq ? q + e * A.q_h : e < HK ? k + (e - A.Hq) * A.k_h : vv + (e - HK) * A.v_h);
+                ro_copy16(&buf[b][i][lane], e < A.Hq ? q + e * A.q_h
+                                            : e < HK ? k + (e - A.Hq) * A.k_h : vv + (e - HK) * A.v_h);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -266,7 +257,7 @@ __global__ void __launch_bounds__(RO_THREADS, RO_BLOCKS) rotary_warp_kernel(cons
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float2 a = unpack2<T>(w[j]);
-                        w[j] = ro_pack<T>(a.x * c[j] - a.y * s[j], a.y * c[j] + a.x * s[j]);
+                        w[j] = pack2<T>(a.x * c[j] - a.y * s[j], a.y * c[j] + a.x * s[j]);
                     }
                 } else {
                     const uint4 p = x[hv];
@@ -274,8 +265,8 @@ __global__ void __launch_bounds__(RO_THREADS, RO_BLOCKS) rotary_warp_kernel(cons
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float2 a = unpack2<T>(w[j]), d = unpack2<T>(o[j]);
-                        w[j] = ro_pack<T>(a.x * c[2 * j] - d.x * s[2 * j], a.y * c[2 * j + 1] - d.y * s[2 * j + 1]);
-                        o[j] = ro_pack<T>(d.x * c[2 * j] + a.x * s[2 * j], d.y * c[2 * j + 1] + a.y * s[2 * j + 1]);
+                        w[j] = pack2<T>(a.x * c[2 * j] - d.x * s[2 * j], a.y * c[2 * j + 1] - d.y * s[2 * j + 1]);
+                        o[j] = pack2<T>(d.x * c[2 * j] + a.x * s[2 * j], d.y * c[2 * j + 1] + a.y * s[2 * j + 1]);
                     }
                     *reinterpret_cast<uint4 *>(y + half + u * 8) = make_uint4(o[0], o[1], o[2], o[3]);
                 }

@@ -207,8 +207,8 @@ __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// One block, or a cluster of `blocks` (0: one block, for the requests alone). The searches and the walks up the parents are chains of dependent reads, so what
-// they read is brought to shared memory first.
+// One block, or a cluster of `blocks` (0: one block, for the requests alone). The searches and the walks up the parents
+// are chains of dependent reads, so what they read is brought to shared memory first.
 __global__ void __launch_bounds__(1024) step_tables_kernel(StepArgs A, int blocks) {
     extern __shared__ int sm[];   // [3][B] prefix sums, then the parents of 63 + blockDim.x rows
     int *cu = sm, *par = sm + 3 * A.B;

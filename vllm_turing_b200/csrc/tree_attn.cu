@@ -6,8 +6,8 @@
 // it sees, 0 where it sees none. A key in a block whose table entry is out of range is not seen.
 //
 // Rows: the n tokens x G = Hq / Hkv query heads of one cached head share its keys, so they are the rows of one product,
-// whole tokens of up to 128 rows to a tile (tcgen05 M = 128; unused rows cost nothing that counts, since rows are independent and the stream of
-// keys bounds the kernel below about 250 rows). Per tile of TK keys:
+// whole tokens of up to 128 rows to a tile (tcgen05 M = 128; unused rows cost nothing that counts, since rows are
+// independent and the stream of keys bounds the kernel below about 250 rows). Per tile of TK keys:
 //   S [128, TK] = Q K^T       tcgen05 kind::f16, both K-major, 128-byte swizzle
 //   P = 2^(S scale log2 e - m) in 16 bits, written over S in tensor memory; m, l: running maximum and sum (32 bits)
 //   O [128, D] += P V         tcgen05 kind::f16, P from tensor memory, V from shared memory as it lies in the cache
@@ -35,7 +35,8 @@
 // CTA: the first warps hold rows; one warp each loads K and V tiles by TMA through the block table (a box holds a power
 // of two of rows that divides block_size, so no box crosses a page), a lane per box, into two rings; one issues the
 // MMAs; one fetches the next item's Q. The K warp walks the CTA's range and leaves each segment (an item's tiles in the
-// range) in shared memory for the others. The score MMA of tile t + 1 runs while the softmax of tile t does. Every wait is bounded.
+// range) in shared memory for the others. The score MMA of tile t + 1 runs while the softmax of tile t does. Every wait
+// is bounded.
 //
 // What nothing sees must not matter, whatever the memory holds: scores are selected, not added to; in the tiles that
 // reach past ctx the rows of V past L are set to zero in shared memory, and infinities and NaN in the step's own rows
@@ -75,7 +76,8 @@ template <int NCH, int REP> struct TaLayout {        // NCH: 64-value chunks of 
     // the 7 that fit, or of 12) + 2, which is how far the K warp can be ahead of the rows
     static constexpr int RING = SLOT >= 32768 ? 8 : 16;
     // barriers and small shared state, bytes (checked in the kernel)
-    static constexpr int BARS = ((2 * MAX_SLOTS + 12 + RING) * 8 + RING * 56 + 40 + GR * 1024 + (7 + RING) * 4 + 127) / 128 * 128;
+    static constexpr int BARS =
+        ((2 * MAX_SLOTS + 12 + RING) * 8 + RING * 56 + 40 + GR * 1024 + (7 + RING) * 4 + 127) / 128 * 128;
     // tensor memory: O | S0 S1 | P0 P1 or Q
     static constexpr int S_COL = DP, Q_COL = S_COL + 2 * TK, P_COL = QT ? S_COL : Q_COL, P_LD = QT ? TK : TK / 2;
     static_assert(Q_COL + (QT ? DP / 2 : TK) <= 512, "tensor memory");
@@ -109,7 +111,7 @@ struct TaArgs {
 // What the joining kernel needs to know of the item that CTA c's range starts inside of.
 struct TaDesc {
     int split;               // 1: c's range starts inside an item and c is the first to do so
-    int first, parts;        // slot of the item's first part; CTAs that hold parts (then c, c + 1, ..: slots 2 c, 2 c + 2, ..)
+    int first, parts;        // slot of the item's first part; CTAs that hold parts (then c, c + 1, ..: 2 c, 2 c + 2, ..)
     int tokens, tok0, h;     // the item's tokens, the first one's row, cached head
 };
 
@@ -243,15 +245,6 @@ __device__ __forceinline__ float ta_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-template <typename T> __device__ __forceinline__ uint32_t ta_pack(float a, float b);
-template <> __device__ __forceinline__ uint32_t ta_pack<__half>(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <> __device__ __forceinline__ uint32_t ta_pack<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
 }
 template <typename T> __device__ __forceinline__ bool ta_wild(uint32_t half) {
     constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
@@ -673,8 +666,8 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                     const int c = i / (rows * 64), r = i / 64 % rows, d = i % 64, t = r / A.G, tok = tok0 + t;
                     T x = f2t<T>(0.0f);
                     if ((c0 + c) * 64 + d < A.D && tok >= 0 && tok < A.T)
-                        x = reinterpret_cast<const T *>(A.q)[(long long)tok * A.q_t + (long long)(h0 + r - t * A.G) * A.q_h +
-                                                             (c0 + c) * 64 + d];
+                        x = reinterpret_cast<const T *>(A.q)[(long long)tok * A.q_t +
+                                                             (long long)(h0 + r - t * A.G) * A.q_h + (c0 + c) * 64 + d];
                     reinterpret_cast<T *>(buf + c * (Lay::RR * 128) + r * 128 + (((d >> 3) ^ (r & 7)) << 4))[d & 7] = x;
                 }
                 fence_proxy_async();
@@ -807,7 +800,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
 #pragma unroll
                     for (int j = 0; j < CPT; ++j) mx[j & 3] = fmaxf(mx[j & 3], x[j]);
                     float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    if (GR == 2) {   // the two warps that hold these rows (and have read their scores: P may go over them)
+                    if (GR == 2) {   // the two warps that hold these rows (and have read their scores: P may go there)
                         hm[buf][grp][row] = top;
                         named_sync(TC_EPI_BAR + 1 + q4, 64);
                         top = fmaxf(top, hm[buf][grp ^ 1][row]);
@@ -842,7 +835,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                         const float b = ta_exp2(__fmaf_rn(x[j + 1], A.sl2, off));
                         sum[j & 2] += a;
                         sum[(j & 2) + 1] += b;
-                        w[j >> 1] = ta_pack<T>(a, b);
+                        w[j >> 1] = pack2<T>(a, b);
                     }
                     // P's columns are free: sfull was committed after the MMAs that read them two tiles ago
                     if constexpr (REP == 1) ta_st<CPT / 2>(p_col + (uint32_t)(part * (CPT / 2)), w);
@@ -971,7 +964,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                 }
                 uint32_t w[NV / 2 < 12 ? 12 : NV / 2];
 #pragma unroll
-                for (int e = 0; e < NV / 2; ++e) w[e] = ta_pack<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
+                for (int e = 0; e < NV / 2; ++e) w[e] = pack2<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
 #pragma unroll
                 for (int e = 0; e < NV; e += 8) {
                     if (c + e >= A.D) break;
@@ -983,7 +976,8 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                         }
                     }
                     if (A.o_vec) {
-                        *reinterpret_cast<uint4 *>(dst + c + e) = make_uint4(w[e / 2], w[e / 2 + 1], w[e / 2 + 2], w[e / 2 + 3]);
+                        *reinterpret_cast<uint4 *>(dst + c + e) =
+                            make_uint4(w[e / 2], w[e / 2 + 1], w[e / 2 + 2], w[e / 2 + 3]);
                     } else {
                         uint16_t *d16 = reinterpret_cast<uint16_t *>(dst + c + e);
 #pragma unroll
@@ -996,9 +990,9 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             };
             if constexpr (REP > 1) {
                 // The replicas' sums through shared memory, `width` columns at a time; a thread then adds up the REP
-                // replicas of width / REP of its row's. 32 columns fit the staging area; when the CTA has no further item,
-                // the K and V rings are idle and hold them all. (One loop for both: this runs once per item, from a cold
-                // instruction cache.)
+                // replicas of width / REP of its row's. 32 columns fit the staging area; when the CTA has no further
+                // item, the K and V rings are idle and hold them all. (One loop for both: this runs once per item, from
+                // a cold instruction cache.)
                 const int width = has ? 32 : DP, ld = width + 4;
                 float *area = has ? stage : reinterpret_cast<float *>(kring);
 #pragma unroll 1
@@ -1007,8 +1001,9 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                     for (int c = 0; c < width; c += 64) {
                         float o[64];
                         const bool two = c + 32 < width;
-                        tmem_ld32(lane_base + (uint32_t)(c0 + c), *reinterpret_cast<uint32_t(*)[32]>(o));
-                        if (two) tmem_ld32(lane_base + (uint32_t)(c0 + c + 32), *reinterpret_cast<uint32_t(*)[32]>(o + 32));
+                        const uint32_t col = lane_base + (uint32_t)(c0 + c);
+                        tmem_ld32(col, *reinterpret_cast<uint32_t(*)[32]>(o));
+                        if (two) tmem_ld32(col + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
                         tmem_ld_wait();
                         float4 *y = reinterpret_cast<float4 *>(area + tid * ld + c);
 #pragma unroll
@@ -1037,7 +1032,7 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                     }
                     if (has) named_sync(TC_EPI_BAR, 128);
                 }
-              if (!whole && mine && part == 0) A.stats[slot * TA_ROWS + row] = make_float2(m, l);
+                if (!whole && mine && part == 0) A.stats[slot * TA_ROWS + row] = make_float2(m, l);
             } else if (warp_live) {
                 constexpr int SHARE = DP / GR;   // a group's share of the columns
 #pragma unroll 1
@@ -1118,7 +1113,8 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
                     for (int j = wr; j < d.parts; j += wpr) {
                         const size_t s = j == 0 ? d.first : 2 * (c - 1 + j);
                         const float2 st = A.stats[s * TA_ROWS + r];
-                        const float4 *p = reinterpret_cast<const float4 *>(A.parts) + (s * (DP / 4) + cb * 2) * TA_ROWS + r;
+                        const float4 *p =
+                            reinterpret_cast<const float4 *>(A.parts) + (s * (DP / 4) + cb * 2) * TA_ROWS + r;
                         const float4 a = p[0], b = p[TA_ROWS];
                         const float v[TJ_COLS] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
                         const float mn = fmaxf(m, st.x), mz = mn == -INFINITY ? 0.0f : mn;
@@ -1144,7 +1140,8 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
                         m = mn;
                         l = l * f + g * st.y;
 #pragma unroll
-                        for (int e = 0; e < TJ_COLS; ++e) acc[e] = ta_scaled(acc[e], f) + ta_scaled(acc_sm[w][e][lane], g);
+                        for (int e = 0; e < TJ_COLS; ++e)
+                            acc[e] = ta_scaled(acc[e], f) + ta_scaled(acc_sm[w][e][lane], g);
                     }
                 }
                 __syncthreads();
@@ -1153,7 +1150,7 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             uint32_t w[TJ_COLS / 2];
 #pragma unroll
-            for (int e = 0; e < TJ_COLS / 2; ++e) w[e] = ta_pack<T>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+            for (int e = 0; e < TJ_COLS / 2; ++e) w[e] = pack2<T>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
             if (cb * TJ_COLS >= A.D) continue;
             if (A.o_vec) {
                 *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -1199,7 +1196,8 @@ static bool ta_map(CUtensorMap *m, const void *base, int D, int bs, int Hkv, int
 }
 
 // q [T][Hq][D]; a box is 64 values of the G heads of one cached head, for an item's tokens.
-static bool ta_q_map(CUtensorMap *m, const void *base, int D, int Hq, int T, long long sh, long long st, int G, int tokens) {
+static bool ta_q_map(CUtensorMap *m, const void *base, int D, int Hq, int T, long long sh, long long st, int G,
+                     int tokens) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
     cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)Hq, (cuuint64_t)T};
@@ -1244,14 +1242,17 @@ static int launch_ta(const CUtensorMap &mk, const CUtensorMap &mv, const CUtenso
 }
 
 template <typename T, int NCH>
-static int dispatch_rep(const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mq, const TaArgs &A, cudaStream_t s) {
+static int dispatch_rep(const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mq, const TaArgs &A,
+                        cudaStream_t s) {
     const int rows = A.max_new * A.G;
     if (rows <= 32) return launch_ta<T, NCH, 4>(mk, mv, mq, A, s);
     if (rows <= 64) return launch_ta<T, NCH, 2>(mk, mv, mq, A, s);
     return launch_ta<T, NCH, 1>(mk, mv, mq, A, s);
 }
 
-template <typename T> static int dispatch_ta(const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mq, const TaArgs &A, cudaStream_t s) {
+template <typename T>
+static int dispatch_ta(const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mq, const TaArgs &A,
+                       cudaStream_t s) {
     if (A.D <= 64) return dispatch_rep<T, 1>(mk, mv, mq, A, s);
     if (A.D <= 128) return dispatch_rep<T, 2>(mk, mv, mq, A, s);
     if (A.D <= 192) return dispatch_rep<T, 3>(mk, mv, mq, A, s);
@@ -1276,8 +1277,8 @@ int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, v
                       long long num_blocks, int block_size, float scale, int dtype, void *workspace, size_t ws_bytes,
                       void *stream) {
     if (!q || !k_cache || !v_cache || !out || !strides || !block_table || !cu || !seq_lens || B < 1 || T < 0 ||
-        max_new < 1 || max_new > TA_MAX_NEW || Hkv < 1 || Hq < Hkv || Hq % Hkv || Hq / Hkv > TA_ROWS || D < 8 || D > 256 ||
-        D % 8 || block_size < 8 || block_size % 8 || table_width < 1 || num_blocks < 1 || num_blocks > 0x7ffffffe ||
+        max_new < 1 || max_new > TA_MAX_NEW || Hkv < 1 || Hq < Hkv || Hq % Hkv || Hq / Hkv > TA_ROWS || D < 8 ||
+        D > 256 || D % 8 || block_size < 8 || block_size % 8 || table_width < 1 || num_blocks < 1 || num_blocks > 0x7ffffffe ||
         (dtype != 0 && dtype != 1) || !workspace || ((uintptr_t)workspace & 255) ||
         ws_bytes < vt_tree_attention_ws_bytes(max_new, Hq, Hkv, D) || ((uintptr_t)k_cache & 15) ||
         ((uintptr_t)v_cache & 15) || !(scale == scale))

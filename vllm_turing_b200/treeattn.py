@@ -72,10 +72,11 @@ def tree_attention(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask
     B = tshape[0]
     qs, ks, vs, ts = q.stride(), k_cache.stride(), v_cache.stride(), block_table.stride()
     if not (qs[2] == 1 and 8 <= D <= 256 and D & 7 == 0 and v_cache.shape == cshape and cshape[3] == D and nb >= 1
-            and bs >= 8 and bs & 7 == 0 and 1 <= Hkv <= Hq <= MAX_GROUP * Hkv and Hq % Hkv == 0 and _aligned(k_cache, ks)
-            and _aligned(v_cache, vs) and 1 <= max_new <= MAX_NEW and vector(seq_lens, torch.int32, B)
-            and vector(cu, torch.int32, B + 1) and block_table.dtype == torch.int32
-            and (ts[1] == 1 or tshape[1] == 1) and tshape[1] >= 1 and (mask is None or vector(mask, torch.int64, T))) and T > 0:
+            and bs >= 8 and bs & 7 == 0 and 1 <= Hkv <= Hq <= MAX_GROUP * Hkv and Hq % Hkv == 0
+            and _aligned(k_cache, ks) and _aligned(v_cache, vs) and 1 <= max_new <= MAX_NEW
+            and vector(seq_lens, torch.int32, B) and vector(cu, torch.int32, B + 1)
+            and block_table.dtype == torch.int32 and (ts[1] == 1 or tshape[1] == 1) and tshape[1] >= 1
+            and (mask is None or vector(mask, torch.int64, T))) and T > 0:
         _refuse(q, k_cache, v_cache, block_table, cu, seq_lens, max_new, mask)
     dt, dev = q.dtype, q.device
     if out is None:
