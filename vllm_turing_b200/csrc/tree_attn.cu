@@ -42,8 +42,10 @@
 // reach past ctx the rows of V past L are set to zero in shared memory, and infinities and NaN in the step's own rows
 // are taken out there (0 x inf is NaN) and added to the rows that see them at the end. Those of the context stay: every
 // row sees them. But a weight may be 0 in the products where it is not by definition (a replica's for the keys of the
-// others, one that underflows), so a sum that came out as NaN has its column of the context looked through, and takes
-// the sum of the infinities and NaN found there (ta_context_wild). That costs nothing where sums are finite.
+// others, one that underflows), so where a sum came out as NaN the context is looked through, and the value becomes the
+// sum of the infinities and NaN found there (ta_fix_wild; the joining kernel does the same with its parts). Where sums
+// are finite that costs adding them up: 64 ragged trees 208 -> 211 us, 256 single tokens 341 -> 345 us, one token 12.9 ->
+// 13.3 us on the device. (Looking at each value for itself before it is written: 13.8 us for one token.)
 #include <math.h>
 
 #include "tc_core.cuh"
@@ -373,39 +375,57 @@ __device__ __forceinline__ uint32_t ta_seen(unsigned long long see, int kk0, int
     return jj < 64 ? (uint32_t)(see >> jj) : 0u;
 }
 
-// Bit e of x and of y: some value of column c + e, of the keys j0 .. j1 - 1 of request b and cached head h, is +inf and
-// is -inf; a NaN counts as both. Called by whole warps on uniform values; the lanes share out the keys.
-template <typename T, int NV>
-__device__ __noinline__ uint2 ta_context_wild(const TaArgs &A, int b, int h, int j0, int j1, int c) {
+// After an item's values are written, by whole warps some of whose rows got a NaN that is not their scores': where the
+// context that the segment covers (keys j0 .. j1 - 1 of request b, cached head h) holds infinities or NaN, every row's
+// value is their sum and that of the wild values of the step's own tokens it sees (wn). The lanes share out the keys, for
+// 8 columns at a time: those of the warp, `share` from part * share on of every `width`. parts: the segment is a part of
+// the item, and this row's values are TA_ROWS apart there, by fours; else they are at dst.
+template <typename T>
+__device__ __noinline__ void ta_fix_wild(const TaArgs &A, int b, int h, int j0, int j1, int width, int share, int part,
+                                         int ctx, int seg_k0, int seg_k1, unsigned long long wn, bool ok, T *dst,
+                                         float *parts) {
     constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;   // exponent; the mantissa is below it
     const int *trow = A.table + (long long)b * A.table_stride;
-    uint32_t pos = 0, neg = 0;
-    for (int j = j0 + (int)(threadIdx.x & 31); j < j1; j += 32) {
-        const int page = j / A.bs;
-        if (page >= A.width) break;
-        const int blk = trow[page];
-        if (blk < 0 || blk >= A.num_blocks) continue;
-        const T *v = reinterpret_cast<const T *>(A.v) + blk * A.v_b + (j - page * A.bs) * A.v_r + h * A.v_h + c;
-#pragma unroll
-        for (int i = 0; i < NV / 8; ++i) {
-            if (c + 8 * i >= A.D) break;
-            const uint4 x = *reinterpret_cast<const uint4 *>(v + 8 * i);
+    auto values = [&](int j) -> const T * {   // of key j; null if its page is not there
+        const int page = j / A.bs, blk = page < A.width ? trow[page] : -1;
+        if (blk < 0 || blk >= A.num_blocks) return nullptr;
+        return reinterpret_cast<const T *>(A.v) + blk * A.v_b + (j - page * A.bs) * A.v_r + h * A.v_h;
+    };
+#pragma unroll 1
+    for (int c = 0; c < A.D; c += 8) {
+        if (c % width / share != part) continue;
+        uint32_t pos = 0, neg = 0;   // bit e: column c + e holds +inf, -inf; NaN counts as both
+        for (int j = j0 + (int)(threadIdx.x & 31); j < j1; j += 32) {
+            const T *v = values(j);
+            if (!v) continue;
+            const uint4 x = *reinterpret_cast<const uint4 *>(v + c);
             const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const uint32_t u = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
                 if ((u & E) != E) continue;
                 const bool nan = (u & (E ^ 0x7fffu)) != 0;
-                if (nan || !(u & 0x8000u)) pos |= 1u << (8 * i + e);
-                if (nan || (u & 0x8000u)) neg |= 1u << (8 * i + e);
+                if (nan || !(u & 0x8000u)) pos |= 1u << e;
+                if (nan || (u & 0x8000u)) neg |= 1u << e;
             }
         }
+        pos = __reduce_or_sync(0xffffffffu, pos);
+        neg = __reduce_or_sync(0xffffffffu, neg);
+        for (uint32_t left = ok ? pos | neg : 0u; left; left &= left - 1) {
+            const int e = __ffs((int)left) - 1;
+            float sum = !((neg >> e) & 1u) ? INFINITY : !((pos >> e) & 1u) ? -INFINITY : NAN;
+            for (unsigned long long own = wn; own; own &= own - 1) {
+                const int j = ctx + __ffsll((long long)own) - 1;
+                const T *v = j >= seg_k0 && j < seg_k1 ? values(j) : nullptr;
+                const float f = v ? t2f<T>(v[c + e]) : 0.0f;
+                if (!isfinite(f)) sum += f;
+            }
+            if (parts) parts[(c + e) / 4 * (TA_ROWS * 4) + (c + e) % 4] = sum;
+            else dst[c + e] = f2t<T>(sum);
+        }
+        __syncwarp();
     }
-    return make_uint2(__reduce_or_sync(0xffffffffu, pos), __reduce_or_sync(0xffffffffu, neg));
 }
-
-// x f for a weight f that is 0 only by underflow: an infinity stays one
-__device__ __forceinline__ float ta_scaled(float x, float f) { return isfinite(x) ? x * f : x; }
 
 // ---- the kernel ------------------------------------------------------------------------------------------------------
 template <typename T, int NCH, int REP>
@@ -924,21 +944,13 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
             T *dst = reinterpret_cast<T *>(A.out) + (long long)tok * A.o_t +
                      (long long)(sg.h * A.G + row - row_i * A.G) * A.o_h;
             // NV values of the row from column c: the parts go to the workspace in 32 bits, a whole item's to the output.
-            // All lanes of the warp call it; `ok` is false where the row is none.
-            auto put = [&](auto &o, int c, bool ok) {
+            float odd = 0.0f;   // the sum of what was written: NaN if any of it is (or infinities of both signs are)
+            auto put = [&](auto &o, int c) {
                 constexpr int NV = sizeof(o) / sizeof(float);
-                bool nan = false;
+                float x[4] = {o[0], o[1], o[2], o[3]};
 #pragma unroll
-                for (int e = 0; e < NV; ++e) nan |= o[e] != o[e];
-                if (__any_sync(0xffffffffu, ok && nan && l == l)) {   // (scores that are NaN make l, and the row, NaN)
-                    const uint2 f = ta_context_wild<T, NV>(A, sg.b, sg.h, kt0 * TK, min(ctx, (kt0 + N) * TK), c);
-#pragma unroll
-                    for (int e = 0; e < NV; ++e) {
-                        const bool p = (f.x >> e) & 1u, n = (f.y >> e) & 1u;
-                        if (p || n) o[e] = p && n ? NAN : p ? INFINITY : -INFINITY;
-                    }
-                }
-                if (!ok) return;
+                for (int e = 4; e < NV; ++e) x[e & 3] += o[e];
+                odd += (x[0] + x[1]) + (x[2] + x[3]);
                 if (wn) {   // the values taken out above, for the rows that see them
                     for (unsigned long long left = wn; left; left &= left - 1) {
                         const int j = ctx + __ffsll((long long)left) - 1, page = j / A.bs;
@@ -1015,11 +1027,10 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                         }
                     }
                     named_sync(TC_EPI_BAR, 128);
-                    const bool ok = mine && !dead;
+                    if (mine && !dead) {
 #pragma unroll 2
-                    for (int c = part * (width / REP); c < (part + 1) * (width / REP); c += 8) {
-                        float r[8] = {};
-                        if (ok) {
+                        for (int c = part * (width / REP); c < (part + 1) * (width / REP); c += 8) {
+                            float r[8] = {};
 #pragma unroll
                             for (int k = 0; k < REP; ++k) {
                                 const float4 *y = reinterpret_cast<const float4 *>(area + (k * RR + row) * ld + c);
@@ -1027,8 +1038,8 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                                 r[0] += a.x, r[1] += a.y, r[2] += a.z, r[3] += a.w;
                                 r[4] += b.x, r[5] += b.y, r[6] += b.z, r[7] += b.w;
                             }
+                            put(r, c0 + c);
                         }
-                        put(r, c0 + c, ok);
                     }
                     if (has) named_sync(TC_EPI_BAR, 128);
                 }
@@ -1040,9 +1051,15 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
                     float o[32];
                     tmem_ld32(lane_base + (uint32_t)c, *reinterpret_cast<uint32_t(*)[32]>(o));
                     tmem_ld_wait();
-                    put(o, c, mine && !dead);
+                    if (mine && !dead) put(o, c);
                 }
                 if (!whole && mine && grp == 0) A.stats[slot * TA_ROWS + row] = make_float2(m, l);
+            }
+            if (__any_sync(0xffffffffu, odd != odd && l == l)) {   // (scores that are NaN make l, and the row, NaN)
+                const int width = REP > 1 && has ? 32 : DP, k0 = kt0 * TK, k1 = (kt0 + N) * TK;
+                float *at = A.parts + (slot * (DP / 4) * TA_ROWS + row) * 4;
+                ta_fix_wild<T>(A, sg.b, sg.h, k0, min(ctx, k1), width, width / (REP * GR), part, ctx, k0, k1, wn,
+                               mine && !dead && l == l, dst, whole ? nullptr : at);
             }
             if constexpr (REP > 1) {   // the staging area is the Q buffer again, which the next copy writes
                 fence_proxy_async();
@@ -1067,6 +1084,20 @@ __global__ void __launch_bounds__(TaLayout<NCH, REP>::THREADS, 1)
 // tasks (one token over a long context is cut into many parts). A row's contributors are the CTAs c - 1 .. c1 in order;
 // the warps' sums add up in warp order.
 constexpr int TJ_THREADS = 256, TJ_WARPS = TJ_THREADS / 32, TJ_COLS = 8;
+
+// Column col of row r of the item that CTA c's range starts inside of, when some of the row's are NaN: a value that is
+// infinite or NaN in parts is the sum of those parts, whatever their weights (one that is 0 is so by underflow).
+template <int DP> __device__ __noinline__ float tj_fix_wild(const TaArgs &A, int c, int r, int col, float joined) {
+    const TaDesc d = A.desc[c];
+    float sum = 0.0f;
+    for (int j = 0; j < d.parts; ++j) {
+        const size_t s = j == 0 ? d.first : 2 * (c - 1 + j);
+        const float x = A.parts[((s * (DP / 4) + col / 4) * TA_ROWS + r) * 4 + col % 4];
+        if (!isfinite(x)) sum += x;
+    }
+    return isfinite(sum) ? joined : sum;
+}
+
 template <typename T, int NCH>
 __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_constant__ TaArgs A, int ctas) {
     constexpr int DP = NCH * 64, CBS = DP / TJ_COLS;
@@ -1123,7 +1154,7 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
                         l = l * f + w * st.y;
 #pragma unroll
                         for (int e = 0; e < TJ_COLS; ++e)   // (a part that is all hidden from the row holds zeros)
-                            acc[e] = __fmaf_rn(isfinite(v[e]) ? w : 1.0f, v[e], ta_scaled(acc[e], f));
+                            acc[e] = __fmaf_rn(w, v[e], acc[e] * f);
                     }
                 }
             }
@@ -1140,13 +1171,18 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
                         m = mn;
                         l = l * f + g * st.y;
 #pragma unroll
-                        for (int e = 0; e < TJ_COLS; ++e)
-                            acc[e] = ta_scaled(acc[e], f) + ta_scaled(acc_sm[w][e][lane], g);
+                        for (int e = 0; e < TJ_COLS; ++e) acc[e] = acc[e] * f + g * acc_sm[w][e][lane];
                     }
                 }
                 __syncthreads();
             }
             if (!dst || wr > 0) continue;
+            const float odd = ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
+            if (odd != odd && l == l) {
+#pragma unroll
+                for (int e = 0; e < TJ_COLS; ++e)
+                    acc[e] = tj_fix_wild<DP>(A, base + list[item], r, cb * TJ_COLS + e, acc[e]);
+            }
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             uint32_t w[TJ_COLS / 2];
 #pragma unroll
