@@ -183,14 +183,15 @@ int vt_rotary_cache(const void *q, void *q_out, const void *k, const void *v, vo
 
 /* Attention of each request's new tokens q [T, Hq, D] over its seq_lens[b] cached keys, the last cu[b + 1] - cu[b] of
  * which are the new tokens themselves: token i sees every key before those and, of the new tokens, those with their bit
- * set in mask[cu[b] + i] (int64 [T]), or tokens 0 .. i with mask NULL. Softmax in 32 bits; a token that sees no key
- * gets 0; keys in blocks whose table entry is outside [0, num_blocks) are not seen, whatever the cache holds where
- * nothing is seen. Hq a multiple of Hkv, at most 128 times it (query head h reads cached head h / (Hq / Hkv)), D a
- * multiple of 8 up to 256, block_size a multiple of 8, caches 16-byte aligned with strides that are multiples of 8
- * elements, 1 <= max_new <= 64 (tokens of a request past max_new are not computed; rows past cu[B] are left as they
- * were). strides (host, in elements): token and head stride of q and out, then block, row and head stride of k_cache
- * and of v_cache. workspace: vt_tree_attention_ws_bytes bytes, 256-byte aligned, need not be zeroed; calls that may
- * overlap must not share it. */
+ * set in mask[cu[b] + i] (int64 [T]), or tokens 0 .. i with mask NULL. Softmax and sums in 32 bits, weights rounded to
+ * the inputs' type before they multiply values (of at most 2^120 / keys in magnitude); a token that sees no key gets 0;
+ * an infinite value that is seen gives that infinity, or NaN with one of the other sign; keys in blocks whose table
+ * entry is outside [0, num_blocks) are not seen, whatever the cache holds where nothing is seen. Hq a multiple of Hkv,
+ * at most 128 times it (query head h reads cached head h / (Hq / Hkv)), D a multiple of 8 up to 256, block_size a
+ * multiple of 8, caches 16-byte aligned with strides that are multiples of 8 elements, 1 <= max_new <= 64 (tokens of a
+ * request past max_new are not computed; rows past cu[B] are left as they were). strides (host, in elements): token and
+ * head stride of q and out, then block, row and head stride of k_cache and of v_cache. workspace:
+ * vt_tree_attention_ws_bytes bytes, 256-byte aligned, need not be zeroed; calls that may overlap must not share it. */
 size_t vt_tree_attention_ws_bytes(int max_new, int Hq, int Hkv, int D);
 int vt_tree_attention(const void *q, const void *k_cache, const void *v_cache, void *out, const long long *strides,
                       const void *block_table, long long table_stride, int table_width, const void *cu,

@@ -12,9 +12,10 @@ The drop-in replacement for vllm-turing's hot path (vllm_turing/__init__.py:38-7
     CudaCommunicator.all_gather / gather
   - lmhead: the int8 LM head (W8A16: int8 rows converted to 16-bit in tensor memory, tcgen05 kind::f16) and the
     vocabulary-parallel logits gathered in place
-  - steptables / rotary / treeattn: what stands between the QKV projection and o_proj for a step of drafted tokens --
-    block tables, slot maps and tree masks built on the GPU from request lengths; rotary positions, alone or with the
-    write of k and v to the paged cache; attention of chains and trees of tokens over that cache (tcgen05)
+  - steptables / rotary / treeattn: for a step of drafted tokens, between the QKV projection and o_proj -- block tables,
+    slot maps and tree masks built on the GPU from request lengths; rotary positions, alone or with the write of k and v
+    to the paged cache; attention of chains and trees of up to 64 tokens a request over that cache (tcgen05). Norms of
+    q and k per head, gates of the attention's output and the attention of prompts are not among them
   - customar / tailoverlap: the reference's vLLM-side switches on this path
 VLLM_TURING_DISABLE=1 turns everything off. Every module honours the reference's VLLM_TURING_<NAME> switches.
 """

@@ -14,7 +14,12 @@
 //                             (keys x D: the "MN-major" operand)
 // O stays in tensor memory for all tiles; a row's m is raised, and O and l rescaled, only when a tile's maximum passes
 // m by more than 8 (a factor 2^8): the quotient O / l is the same, P stays below 2^8 (fp16 P is held 2^7 times larger,
-// so that small weights keep their bits), and rescaling, which reads and writes all of O, is rare.
+// so that small weights keep their bits), and rescaling, which reads and writes all of O, is rare. (O is a sum before the
+// division: with bf16 values past 2^120 / L in magnitude it can pass 32 bits where the quotient would not.)
+// P has 16 bits because one MMA takes both operands in one type, V's: each weight is rounded once, by at most 2^-8 (bf16)
+// or 2^-11 (fp16) of itself; maxima, l, O and the parts have 32 bits. On random inputs the output's error against 64
+// bits, relative to its norm, is 0.0018 .. 0.0023 in bf16 where the output's own rounding alone gives 0.0017, and 0.00026
+// for 0.00021 in fp16. Weights of 32 bits would take a second product with the remainders.
 //
 // The softmax of a tile must not take longer than its bytes take to arrive (about 2800 cycles for 64 KB of K and V), nor
 // than its products where those bound. A thread holds a row, so with few rows one warp would do all the work; hence
