@@ -154,7 +154,7 @@ def test_a_stack_that_runs_out():
 
 @pytest.mark.parametrize("layout", ["blocks", "heads", "joint"])
 def test_moving_an_accepted_path(layout):
-    """The lines that INTEGRATION.md gives for it, over every layout of a cache that the operators take."""
+    """The lines that the integration guide gives for it, over every layout of a cache that the operators take."""
     import os
     import textwrap
     with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")) as f:
