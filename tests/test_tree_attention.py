@@ -550,3 +550,23 @@ def test_inputs_that_require_a_gradient():
             A.tree_attention(*x, i(2, 5), i(3), i(2), 5)
         with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
             A.tree_attention(*x, i(2, 5), i(3), i(2), 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq, n, D", [(2, 1, 128), (12, 5, 80), (16, 20, 256)])
+def test_a_key_whose_values_are_all_nan(Hq, n, D):
+    """One key's values of one head, or of 8 columns, among infinities before and after it: NaN there and nowhere else."""
+    for L in (40, 1000, 30000):
+        c = make([L + n], [n], Hq, 2, D, 16, torch.bfloat16, seed=L)
+        want = run(c)
+        half = Hq // 2
+        page, at = c["table"][0].long(), [0, L // 3, L // 2, L - 1]
+        c["vc"][page[at[0] // 16], at[0] % 16, 0, 8:24] = float("inf")
+        c["vc"][page[at[1] // 16], at[1] % 16, 0, 8:16] = float("nan")
+        c["vc"][page[at[3] // 16], at[3] % 16, 0, 24:40] = -float("inf")
+        c["vc"][page[at[2] // 16], at[2] % 16, 1] = float("nan")
+        want[:, :half, 8:16], want[:, :half, 16:24], want[:, :half, 24:40] = float("nan"), float("inf"), -float("inf")
+        want[:, half:] = float("nan")
+        out = run(c)
+        assert torch.equal(out.isnan(), want.isnan())
+        assert torch.equal(out.nan_to_num(7.0, 9e9, -9e9), want.nan_to_num(7.0, 9e9, -9e9))

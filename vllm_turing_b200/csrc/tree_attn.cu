@@ -49,8 +49,8 @@
 // row sees them. But a weight may be 0 in the products where it is not by definition (a replica's for the keys of the
 // others, one that underflows), so where a sum came out as NaN the context is looked through, and the value becomes the
 // sum of the infinities and NaN found there (ta_fix_wild; the joining kernel does the same with its parts). Where sums
-// are finite that costs adding them up: 64 ragged trees 208 -> 211 us, 256 single tokens 341 -> 345 us, one token 12.9 ->
-// 13.3 us on the device. (Looking at each value for itself before it is written: 13.8 us for one token.)
+// are finite that costs adding them up: 64 ragged trees 208.6 -> 211.8 us, 256 single tokens 344 -> 347 us, one token
+// 12.8 -> 13.0 us on the device. (Looking at each value for itself before it is written: 13.8 us for one token.)
 #include <math.h>
 
 #include "tc_core.cuh"
@@ -400,22 +400,29 @@ __device__ __noinline__ void ta_fix_wild(const TaArgs &A, int b, int h, int j0, 
     for (int c = 0; c < A.D; c += 8) {
         if (c % width / share != part) continue;
         uint32_t pos = 0, neg = 0;   // bit e: column c + e holds +inf, -inf; NaN counts as both
-        for (int j = j0 + (int)(threadIdx.x & 31); j < j1; j += 32) {
-            const T *v = values(j);
-            if (!v) continue;
-            const uint4 x = *reinterpret_cast<const uint4 *>(v + c);
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        for (int k = j0; k < j1 && (pos & neg) != 0xffu; k += 4 * 32) {   // nothing is added to 8 columns of NaN
+            uint4 x[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t u = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
-                if ((u & E) != E) continue;
-                const bool nan = (u & (E ^ 0x7fffu)) != 0;
-                if (nan || !(u & 0x8000u)) pos |= 1u << e;
-                if (nan || (u & 0x8000u)) neg |= 1u << e;
+            for (int i = 0; i < 4; ++i) {
+                const int j = k + 32 * i + (int)(threadIdx.x & 31);
+                const T *v = j < j1 ? values(j) : nullptr;
+                x[i] = v ? *reinterpret_cast<const uint4 *>(v + c) : make_uint4(0, 0, 0, 0);
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t u = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+                    if ((u & E) != E) continue;
+                    const bool nan = (u & (E ^ 0x7fffu)) != 0;
+                    if (nan || !(u & 0x8000u)) pos |= 1u << e;
+                    if (nan || (u & 0x8000u)) neg |= 1u << e;
+                }
+            }
+            pos = __reduce_or_sync(0xffffffffu, pos);
+            neg = __reduce_or_sync(0xffffffffu, neg);
         }
-        pos = __reduce_or_sync(0xffffffffu, pos);
-        neg = __reduce_or_sync(0xffffffffu, neg);
         for (uint32_t left = ok ? pos | neg : 0u; left; left &= left - 1) {
             const int e = __ffs((int)left) - 1;
             float sum = !((neg >> e) & 1u) ? INFINITY : !((pos >> e) & 1u) ? -INFINITY : NAN;
