@@ -1,8 +1,8 @@
 """Rotary positions of query and key heads (csrc/rotary.cu): pairs by halves or interleaved, part of the head, scaled
 for long contexts; alone (either direction), or in one kernel with the write of k and v to the paged cache.
 
-Angles come from 64-bit frequencies and are reduced in 64 bits, so far positions keep 32-bit accuracy without a table
-of cosines.
+Angles come from 64-bit frequencies and are reduced in 64 bits, so far positions (up to 2^31) keep 32-bit accuracy
+without a table of cosines.
 """
 import math
 import struct
